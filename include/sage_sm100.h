@@ -327,6 +327,80 @@ int sage_flash_attn_varlen_fwd(const void* q, const void* k, const void* v, void
                                const int64_t v_strides[2], const int64_t o_strides[2], int causal, float sm_scale,
                                void* stream);
 
+/* ------------------------------------------------------------------ paged key/value cache
+ * Keys and values of many sequences in pages of page_size tokens (a power of two from 16 to
+ * 1024). Position p of sequence b lives in page page_table[b * table_stride + p / page_size], row
+ * p % page_size; several sequences may share pages. The reference has no cache: these entry points
+ * extend its attention operators (kernels/flash_attn/triton_impl.py:110-128) to serving.
+ *
+ * Arrays that the calls share (device memory, int32):
+ *   page_table  page numbers, pages_per_seq per sequence, rows table_stride entries apart
+ *   seq_lens    [batch]: tokens that sequence b holds, the new ones of this call included
+ *   cu_seqlens  [batch + 1] prefix sums of the new tokens in the packed tensors, or NULL: one new
+ *               token per sequence, row b being sequence b's
+ * New token i of the n of sequence b has position seq_lens[b] - n + i. None of the arrays is
+ * trusted: prefix sums are clamped to the packed tensor, lengths to pages_per_seq pages, and a page
+ * number outside [0, num_pages) is skipped by a write and reads as zeros; so entries that no
+ * position reaches may hold anything. Packed rows behind the last sequence are left as they are.
+ */
+#define SAGE_CACHE_16BIT 0  /* keys and values in `dtype` */
+#define SAGE_CACHE_INT8  1  /* INT8 codes with one fp32 scale per token and head */
+
+typedef struct sage_paged_cache {
+  void* k;               /* [num_pages, heads_kv, page_size, head_dim], any strides */
+  void* v;
+  float* k_scale;        /* [num_pages, heads_kv, page_size] contiguous (SAGE_CACHE_INT8) */
+  float* v_scale;
+  const float* k_mean;   /* [heads_kv, head_dim] or NULL (SAGE_CACHE_INT8): subtracted from K before it
+                            is quantised, added when it is read back; constant for the cache's life */
+  int64_t num_pages, page_size, heads_kv, head_dim;
+  int64_t k_strides[3];  /* elements: page, head, token; multiples of 16 bytes */
+  int64_t v_strides[3];
+  int dtype;             /* SAGE_DTYPE_*: of new tokens, of tokens read back and of attention */
+  int storage;           /* SAGE_CACHE_* */
+} sage_paged_cache;
+
+/*
+ * Write new tokens' keys and values (packed [tokens, heads_kv, head_dim], element strides
+ * {head, token}) into the cache. SAGE_CACHE_INT8 stores, per row x (K: x - k_mean) of head_dim
+ * values, scale = max|x| / 127 and codes rint(127 x / max|x|), ties to even.
+ */
+int sage_paged_append(const sage_paged_cache* cache, const void* k, const void* v, const int64_t k_strides[2],
+                      const int64_t v_strides[2], const int32_t* page_table, int64_t table_stride,
+                      int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch,
+                      int64_t tokens, void* stream);
+
+/*
+ * Read the newest tokens back: packed rows as sage_paged_append takes them, code * scale (+ k_mean)
+ * rounded once to `dtype`. Positions below 0 and bad pages read as zeros.
+ */
+int sage_paged_gather(const sage_paged_cache* cache, void* k, void* v, const int64_t k_strides[2],
+                      const int64_t v_strides[2], const int32_t* page_table, int64_t table_stride,
+                      int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch,
+                      int64_t tokens, void* stream);
+
+/* Bytes of scratch that sage_paged_attn_fwd needs (the partial results of work split along the
+ * keys). Calls that may overlap on the GPU need workspaces of their own. */
+size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q, int64_t batch, int64_t total_q,
+                                  int64_t max_seqlen_q, int64_t pages_per_seq);
+
+/*
+ * Attention of the new tokens' queries over the cache, which already holds their keys and values:
+ * q / o packed [total_q, heads_q, head_dim] with element strides {head, token}; GQA as elsewhere.
+ * The query at position p sees key j < seq_lens[b] when j <= p (causal; all keys otherwise) and,
+ * with window > 0 (causal only), j > p - window or j < sinks. A query that sees no key gives 0.
+ * max_seqlen_q bounds the new tokens of a sequence. o = q (the identical view) is allowed; other
+ * overlaps of o are rejected. Keys and values that no query of a sequence sees may hold anything,
+ * NaN included; a NaN or infinity in a value that one query sees may reach queries of the same
+ * sequence that do not.
+ */
+int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int64_t q_strides[2], void* o,
+                        const int64_t o_strides[2], int64_t heads_q, const int32_t* page_table,
+                        int64_t table_stride, int64_t pages_per_seq, const int32_t* seq_lens,
+                        const int32_t* cu_seqlens, int64_t batch, int64_t total_q, int64_t max_seqlen_q, int causal,
+                        int64_t window, int64_t sinks, float sm_scale, void* workspace, size_t workspace_bytes,
+                        void* stream);
+
 /*
  * Synchronise `stream`, then read and clear the device-side status word of the current
  * device (SAGE_DEV_* bits; 0 = no wait ran out). Returns SAGE_OK, or SAGE_ERR_TIMEOUT

@@ -32,6 +32,19 @@ SAGE_FLAG_QBLK_MASK = 0x700
 SAGE_FLAG_QBLK = {128: 0x000, 64: 0x100, 32: 0x200, 16: 0x300, 1: 0x400}
 
 
+SAGE_CACHE_16BIT = 0
+SAGE_CACHE_INT8 = 1
+
+
+class PagedCacheStruct(ctypes.Structure):
+    """sage_paged_cache of include/sage_sm100.h."""
+    _fields_ = [("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p),
+                ("v_scale", ctypes.c_void_p), ("k_mean", ctypes.c_void_p), ("num_pages", ctypes.c_int64),
+                ("page_size", ctypes.c_int64), ("heads_kv", ctypes.c_int64), ("head_dim", ctypes.c_int64),
+                ("k_strides", ctypes.c_int64 * 3), ("v_strides", ctypes.c_int64 * 3), ("dtype", ctypes.c_int),
+                ("storage", ctypes.c_int)]
+
+
 def qblk_flag(blkq: int) -> int:
     """SAGE_FLAG_QBLK_* bits for a Q block of `blkq` rows (128, 64, 32, 16 or 1)."""
     if blkq not in SAGE_FLAG_QBLK:
@@ -46,6 +59,7 @@ _I = ctypes.c_int
 _U = ctypes.c_uint
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
+_PC = ctypes.POINTER(PagedCacheStruct)
 SIGNATURES = {
     "sage_abi_version": (_I, []),
     "sage_last_error": (ctypes.c_char_p, []),
@@ -73,6 +87,11 @@ SIGNATURES = {
                              _I64P, _I64P, _I64P, _I64P, _I, _F, _I, _U, _P, _P, _P, _P, _P, _P, _P, _P, _SZ, _P]),
     "sage_flash_attn_varlen_fwd": (_I, [_P, _P, _P, _P, _I, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P,
                                         _I64P, _I64P, _I64P, _I64P, _I, _F, _P]),
+    "sage_paged_append": (_I, [_PC, _P, _P, _I64P, _I64P, _P, _I64, _I64, _P, _P, _I64, _I64, _P]),
+    "sage_paged_gather": (_I, [_PC, _P, _P, _I64P, _I64P, _P, _I64, _I64, _P, _P, _I64, _I64, _P]),
+    "sage_paged_workspace_bytes": (_SZ, [_PC, _I64, _I64, _I64, _I64, _I64]),
+    "sage_paged_attn_fwd": (_I, [_PC, _P, _I64P, _P, _I64P, _I64, _P, _I64, _I64, _P, _P, _I64, _I64, _I64, _I, _I64,
+                                 _I64, _F, _P, _SZ, _P]),
     "sage_device_status": (_I, [ctypes.POINTER(ctypes.c_int), _P]),
     "sage_watchdog_selftest": (_I, [_U, _P]),
 }

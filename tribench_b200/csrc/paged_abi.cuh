@@ -1,0 +1,277 @@
+// paged_abi.cuh — the C entry points of the paged cache (include/sage_sm100.h): validation, tensor
+// maps and launches. Included by sage_abi.cu, whose helpers it uses.
+#pragma once
+
+namespace {
+
+int check_cache(const sage_paged_cache* c) {
+  if (!c) return fail(SAGE_ERR_INVALID_ARG, "cache is NULL");
+  if (c->dtype != SAGE_DTYPE_F16 && c->dtype != SAGE_DTYPE_BF16)
+    return fail(SAGE_ERR_INVALID_ARG, "dtype %d is neither SAGE_DTYPE_F16 nor SAGE_DTYPE_BF16", c->dtype);
+  if (c->storage != SAGE_CACHE_16BIT && c->storage != SAGE_CACHE_INT8)
+    return fail(SAGE_ERR_INVALID_ARG, "cache storage %d unknown", c->storage);
+  if (c->head_dim != 64 && c->head_dim != 128)
+    return fail(SAGE_ERR_INVALID_ARG, "head_dim %lld unsupported (64 or 128)", (long long)c->head_dim);
+  const int64_t P = c->page_size;
+  if (P < 16 || P > 1024 || (P & (P - 1)))
+    return fail(SAGE_ERR_INVALID_ARG, "page_size %lld is not a power of two from 16 to 1024", (long long)P);
+  if (c->num_pages <= 0 || c->num_pages > (1LL << 31) - 1 || c->heads_kv <= 0 || c->heads_kv > 65535)
+    return fail(SAGE_ERR_INVALID_ARG, "empty or oversized cache: num_pages=%lld heads_kv=%lld",
+                (long long)c->num_pages, (long long)c->heads_kv);
+  const bool i8 = c->storage == SAGE_CACHE_INT8;
+  const int64_t unit = i8 ? 16 : 8;  // elements of 16 bytes
+  for (int i = 0; i < 3; ++i) {
+    if (c->k_strides[i] <= 0 || c->k_strides[i] % unit || c->v_strides[i] <= 0 || c->v_strides[i] % unit)
+      return fail(SAGE_ERR_INVALID_ARG, "cache stride[%d] (k %lld, v %lld) must be a positive multiple of %lld elements",
+                  i, (long long)c->k_strides[i], (long long)c->v_strides[i], (long long)unit);
+    if (c->k_strides[i] > (1LL << 38) || c->v_strides[i] > (1LL << 38))
+      return fail(SAGE_ERR_INVALID_ARG, "cache stride[%d] is too large", i);
+  }
+  if (!c->k || !c->v || (i8 && (!c->k_scale || !c->v_scale))) return fail(SAGE_ERR_INVALID_ARG, "NULL cache pointer");
+  if (!i8 && (c->k_scale || c->v_scale || c->k_mean))
+    return fail(SAGE_ERR_INVALID_ARG, "scales and k_mean belong to an INT8 cache");
+  if (!aligned16(c->k) || !aligned16(c->v) || !aligned16(c->k_scale) || !aligned16(c->v_scale) || !aligned16(c->k_mean))
+    return fail(SAGE_ERR_INVALID_ARG, "cache tensors must be 16-byte aligned");
+  return SAGE_OK;
+}
+
+// Checks what append, gather and attention share, and fills the device-side description.
+int paged_seqs(const sage_paged_cache* c, const int32_t* page_table, int64_t table_stride, int64_t pages_per_seq,
+               const int32_t* seq_lens, const int32_t* cu, int64_t batch, int64_t tokens, int64_t max_new,
+               sage::PagedSeqs* s) {
+  if (batch > 0 && (!page_table || !seq_lens)) return fail(SAGE_ERR_INVALID_ARG, "page_table or seq_lens is NULL");
+  if (((reinterpret_cast<uintptr_t>(page_table) | reinterpret_cast<uintptr_t>(seq_lens) |
+        reinterpret_cast<uintptr_t>(cu)) & 3u) != 0)
+    return fail(SAGE_ERR_INVALID_ARG, "page_table, seq_lens and cu_seqlens must be 4-byte aligned");
+  if (batch < 0 || tokens < 0 || batch > (1 << 20) || tokens > (1LL << 30))
+    return fail(SAGE_ERR_INVALID_ARG, "batch=%lld or tokens=%lld out of range", (long long)batch, (long long)tokens);
+  if (!cu && tokens != batch)
+    return fail(SAGE_ERR_INVALID_ARG, "without cu_seqlens every sequence has one token: %lld tokens for %lld sequences",
+                (long long)tokens, (long long)batch);
+  if (pages_per_seq <= 0 || pages_per_seq > (1LL << 30) || table_stride < 0 || (batch > 1 && table_stride < pages_per_seq))
+    return fail(SAGE_ERR_INVALID_ARG, "pages_per_seq=%lld and table_stride=%lld do not fit", (long long)pages_per_seq,
+                (long long)table_stride);
+  if (max_new < 1) return fail(SAGE_ERR_INVALID_ARG, "max_seqlen_q=%lld must be positive", (long long)max_new);
+  s->cu = cu; s->lens = seq_lens; s->table = page_table; s->table_stride = table_stride;
+  s->batch = (int)batch; s->width = (int)pages_per_seq; s->tokens = (int)tokens;
+  s->max_new = (int)std::min(max_new, tokens);
+  s->cap = (int)std::min<int64_t>(pages_per_seq * c->page_size, 1LL << 30);
+  return SAGE_OK;
+}
+
+int page_shift(const sage_paged_cache* c) {
+  int s = 0;
+  while ((1LL << s) < c->page_size) ++s;
+  return s;
+}
+
+Span cache_span(const sage_paged_cache* c, bool v) {
+  return tensor_span(v ? c->v : c->k, v ? c->v_strides : c->k_strides, c->num_pages, c->heads_kv, c->page_size,
+                     c->head_dim, c->storage == SAGE_CACHE_INT8 ? 1 : 2);
+}
+Span scale_span(const sage_paged_cache* c, bool v) {
+  return buffer_span(v ? c->v_scale : c->k_scale, static_cast<size_t>(c->num_pages * c->heads_kv * c->page_size) * 4);
+}
+
+template <bool READ>
+int paged_move(const sage_paged_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
+               const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, const int32_t* cu,
+               int64_t batch, int64_t tokens, void* stream) {
+  if (int rc = check_cache(c)) return rc;
+  sage::PagedMoveParams p{};
+  if (int rc = paged_seqs(c, table, table_stride, width, lens, cu, batch, tokens, 1LL << 30, &p.s)) return rc;
+  if (tokens == 0 || batch == 0) return SAGE_OK;
+  int64_t k3[3], v3[3];
+  if (int rc = packed_strides("k", ks, k3)) return rc;
+  if (int rc = packed_strides("v", vs, v3)) return rc;
+  if (!k || !v) return fail(SAGE_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(SAGE_ERR_INVALID_ARG, "k/v must be 16-byte aligned");
+  // what is written must not share a byte with anything else that the call touches
+  const Span sk = tensor_span(k, k3, 1, c->heads_kv, tokens, c->head_dim, 2);
+  const Span sv = tensor_span(v, v3, 1, c->heads_kv, tokens, c->head_dim, 2);
+  const Span held[] = {cache_span(c, false), cache_span(c, true), scale_span(c, false), scale_span(c, true)};
+  for (const Span& h : held)
+    if (spans_overlap(sk, h) || spans_overlap(sv, h))
+      return fail(SAGE_ERR_INVALID_ARG, "k or v overlaps the cache");
+  if (READ && spans_overlap(sk, sv)) return fail(SAGE_ERR_INVALID_ARG, "k and v overlap each other");
+  if (int rc = check_arch()) return rc;
+  p.c.k = c->k; p.c.v = c->v; p.c.k_scale = c->k_scale; p.c.v_scale = c->v_scale; p.c.k_mean = c->k_mean;
+  p.c.k_sp = c->k_strides[0]; p.c.k_sh = c->k_strides[1]; p.c.k_st = c->k_strides[2];
+  p.c.v_sp = c->v_strides[0]; p.c.v_sh = c->v_strides[1]; p.c.v_st = c->v_strides[2];
+  p.c.pages = (int)c->num_pages; p.c.page_shift = page_shift(c); p.c.heads = (int)c->heads_kv;
+  p.k = const_cast<void*>(k); p.v = const_cast<void*>(v);
+  p.k_sh = ks[0]; p.k_st = ks[1]; p.v_sh = vs[0]; p.v_st = vs[1];
+  const unsigned grid = (unsigned)cdiv(tokens, sage::kPagedThreads / 32);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool i8 = c->storage == SAGE_CACHE_INT8, bf = c->dtype == SAGE_DTYPE_BF16;
+#define SAGE_MOVE(D, T, I8) sage::paged_move_kernel<D, T, I8, READ><<<grid, sage::kPagedThreads, 0, st>>>(p)
+#define SAGE_MOVE_T(D)                                                                                   \
+  do {                                                                                                   \
+    if (i8) { if (bf) SAGE_MOVE(D, __nv_bfloat16, true); else SAGE_MOVE(D, __half, true); }              \
+    else SAGE_MOVE(D, __half, false); /* 16-bit values are copied as they are */                         \
+  } while (0)
+  if (c->head_dim == 128) SAGE_MOVE_T(128);
+  else SAGE_MOVE_T(64);
+#undef SAGE_MOVE_T
+#undef SAGE_MOVE
+  SAGE_CUDA_TRY(cudaGetLastError());
+  return SAGE_OK;
+}
+
+// ---------------------------------------------------------------- attention over the cache
+size_t decode_ws_bytes(int64_t D) {
+  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
+  return align256(rows * D * 4) + align256(rows * 4 * 4) + align256(sizeof(int4) * sage::kDecPieces);
+}
+
+// Tensor maps of the cache's K or V ([pages][heads][page][D], boxes of at most `rows` tokens) and of
+// its scales ([pages][heads][page]).
+int cache_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows) {
+  const int64_t* s = v ? c->v_strides : c->k_strides;
+  const void* base = v ? c->v : c->k;
+  const uint32_t box = (uint32_t)std::min<int64_t>(rows, c->page_size);
+  if (c->storage == SAGE_CACHE_INT8)
+    return encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, c->head_dim, c->page_size, c->heads_kv, c->num_pages,
+                     s[2], s[1], s[0], (uint32_t)c->head_dim, box,
+                     c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+  return encode_4d(map, c->dtype == SAGE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                   2, base, c->head_dim, c->page_size, c->heads_kv, c->num_pages, s[2], s[1], s[0], 64, box,
+                   CU_TENSOR_MAP_SWIZZLE_128B);
+}
+int scale_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows) {
+  const int64_t P = c->page_size;
+  return encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, v ? c->v_scale : c->k_scale, P, c->heads_kv, c->num_pages, 1,
+                   P, P * c->heads_kv, P * c->heads_kv * c->num_pages, (uint32_t)std::min<int64_t>(rows, P), 1,
+                   CU_TENSOR_MAP_SWIZZLE_NONE);
+}
+
+struct PagedMaps {
+  CUtensorMap k, v, ks, vs;
+};
+
+template <int D, bool I8, typename T>
+int launch_decode(const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
+  using C = sage::DecodeCfg<D, I8>;
+  auto kern = sage::paged_decode_kernel<D, I8, T>;
+  if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
+  kern<<<sage::kDecPieces, sage::kDecThreads, C::SMEM, st>>>(m.k, m.v, m.ks, m.vs, p);
+  SAGE_CUDA_TRY(cudaGetLastError());
+  // the join starts while the pieces run and waits on the device for all of them
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(sage::kDecPieces, (unsigned)std::min(max_rows, sage::kDecRows));
+  cfg.blockDim = dim3(sage::kCombineThreads);
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  SAGE_CUDA_TRY(cudaLaunchKernelEx(&cfg, sage::paged_combine_kernel<D, I8, T>, p));
+  return SAGE_OK;
+}
+
+template <int D>
+int decode_dispatch(bool i8, bool bf, const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
+  if (i8) return bf ? launch_decode<D, true, __nv_bfloat16>(m, p, max_rows, st)
+                    : launch_decode<D, true, __half>(m, p, max_rows, st);
+  return bf ? launch_decode<D, false, __nv_bfloat16>(m, p, max_rows, st)
+            : launch_decode<D, false, __half>(m, p, max_rows, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+int sage_paged_append(const sage_paged_cache* cache, const void* k, const void* v, const int64_t k_strides[2],
+                      const int64_t v_strides[2], const int32_t* page_table, int64_t table_stride,
+                      int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch,
+                      int64_t tokens, void* stream) {
+  g_last_error.clear();
+  return paged_move<false>(cache, k, v, k_strides, v_strides, page_table, table_stride, pages_per_seq, seq_lens,
+                           cu_seqlens, batch, tokens, stream);
+}
+
+int sage_paged_gather(const sage_paged_cache* cache, void* k, void* v, const int64_t k_strides[2],
+                      const int64_t v_strides[2], const int32_t* page_table, int64_t table_stride,
+                      int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch,
+                      int64_t tokens, void* stream) {
+  g_last_error.clear();
+  return paged_move<true>(cache, k, v, k_strides, v_strides, page_table, table_stride, pages_per_seq, seq_lens,
+                          cu_seqlens, batch, tokens, stream);
+}
+
+size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q, int64_t batch, int64_t total_q,
+                                  int64_t max_seqlen_q, int64_t pages_per_seq) {
+  if (!cache || heads_q <= 0 || batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || pages_per_seq <= 0) return 0;
+  return decode_ws_bytes(cache->head_dim);
+}
+
+int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int64_t q_strides[2], void* o,
+                        const int64_t o_strides[2], int64_t heads_q, const int32_t* page_table, int64_t table_stride,
+                        int64_t pages_per_seq, const int32_t* seq_lens, const int32_t* cu_seqlens, int64_t batch,
+                        int64_t total_q, int64_t max_seqlen_q, int causal, int64_t window, int64_t sinks,
+                        float sm_scale, void* workspace, size_t workspace_bytes, void* stream) {
+  g_last_error.clear();
+  const sage_paged_cache* c = cache;
+  if (int rc = check_cache(c)) return rc;
+  if (heads_q <= 0 || heads_q % c->heads_kv != 0)
+    return fail(SAGE_ERR_INVALID_ARG, "heads_q=%lld is not a multiple of heads_kv=%lld", (long long)heads_q,
+                (long long)c->heads_kv);
+  const int64_t G = heads_q / c->heads_kv;
+  if (window < 0 || sinks < 0) return fail(SAGE_ERR_INVALID_ARG, "window and sinks must not be negative");
+  if (window > 0 && !causal) return fail(SAGE_ERR_INVALID_ARG, "a window needs causal attention");
+  if (sinks > 0 && window == 0) return fail(SAGE_ERR_INVALID_ARG, "sinks need a window");
+  sage::DecodeParams p{};
+  if (int rc = paged_seqs(c, page_table, table_stride, pages_per_seq, seq_lens, cu_seqlens, batch, total_q,
+                          max_seqlen_q, &p.s))
+    return rc;
+  if (total_q * G > (1LL << 30)) return fail(SAGE_ERR_INVALID_ARG, "total_q * heads_q / heads_kv exceeds 2^30");
+  if (total_q == 0 || batch == 0) return SAGE_OK;
+  int64_t qs[3], os[3];
+  if (int rc = packed_strides("q", q_strides, qs)) return rc;
+  if (int rc = packed_strides("o", o_strides, os)) return rc;
+  if (!q || !o) return fail(SAGE_ERR_INVALID_ARG, "NULL tensor pointer");
+  if (!aligned16(q) || !aligned16(o)) return fail(SAGE_ERR_INVALID_ARG, "q/o must be 16-byte aligned");
+  const size_t need = sage_paged_workspace_bytes(c, heads_q, batch, total_q, max_seqlen_q, pages_per_seq);
+  if (!workspace || workspace_bytes < need)
+    return fail(SAGE_ERR_WORKSPACE, "workspace of %zu bytes needed, %zu given", need, workspace_bytes);
+  if (!aligned16(workspace)) return fail(SAGE_ERR_INVALID_ARG, "workspace must be 16-byte aligned");
+  const NamedSpan others[] = {{"k", cache_span(c, false)}, {"v", cache_span(c, true)},
+                              {"k_scale", scale_span(c, false)}, {"v_scale", scale_span(c, true)},
+                              {"workspace", buffer_span(workspace, workspace_bytes)}};
+  if (int rc = check_out_alias(o, os, tensor_span(o, os, 1, heads_q, total_q, c->head_dim, 2), q, qs,
+                               tensor_span(q, qs, 1, heads_q, total_q, c->head_dim, 2), others, 5))
+    return rc;
+  if (int rc = check_arch()) return rc;
+  const bool i8 = c->storage == SAGE_CACHE_INT8, bf = c->dtype == SAGE_DTYPE_BF16;
+  const int64_t D = c->head_dim;
+  PagedMaps m;
+  if (int rc = cache_map(&m.k, c, false, sage::kDecKeys)) return rc;
+  if (int rc = cache_map(&m.v, c, true, sage::kDecKeys)) return rc;
+  m.ks = m.k;
+  m.vs = m.v;
+  if (i8) {
+    if (int rc = scale_map(&m.ks, c, false, sage::kDecKeys)) return rc;
+    if (int rc = scale_map(&m.vs, c, true, sage::kDecKeys)) return rc;
+  }
+  p.q = q; p.o = o;
+  p.q_sh = q_strides[0]; p.q_st = q_strides[1]; p.o_sh = o_strides[0]; p.o_st = o_strides[1];
+  p.Hkv = (int)c->heads_kv; p.G = (int)G;
+  p.page_shift = page_shift(c);
+  p.causal = causal ? 1 : 0;
+  p.window = (int)std::min<int64_t>(window, 1LL << 30);
+  p.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
+  const double s = sm_scale > 0.0f ? static_cast<double>(sm_scale) : 1.0 / std::sqrt(static_cast<double>(D));
+  p.scale_log2 = static_cast<float>(s * 1.4426950408889634);
+  char* w = static_cast<char*>(workspace);
+  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
+  p.part = reinterpret_cast<float*>(w);
+  p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
+  p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
+  p.wait_limit_ns = wait_limit_ns();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, 1 << 20);
+  return D == 128 ? decode_dispatch<128>(i8, bf, m, p, max_rows, st) : decode_dispatch<64>(i8, bf, m, p, max_rows, st);
+}
+
+}  // extern "C"

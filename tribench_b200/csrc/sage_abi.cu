@@ -17,6 +17,8 @@
 
 #include "../../include/sage_sm100.h"
 #include "sage_attn.cuh"
+#include "sage_decode.cuh"
+#include "sage_paged.cuh"
 #include "sage_quant.cuh"
 
 namespace {
@@ -1253,3 +1255,5 @@ int sage_debug_phase_cycles(unsigned long long* host, size_t count) {
 #endif
 
 }  // extern "C"
+
+#include "paged_abi.cuh"

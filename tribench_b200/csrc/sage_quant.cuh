@@ -50,6 +50,13 @@ template <> struct Half8<__half> {
       f[2 * i + 1] = t.y;
     }
   }
+  __device__ static __forceinline__ uint4 from_float(const float (&f)[8]) {
+    uint4 u;
+    __half2* h = reinterpret_cast<__half2*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    return u;
+  }
   // max |h| over the 8 halves, exact (comparisons of 16-bit values), as fp32
   __device__ static __forceinline__ float absmax(const uint4& u) {
     const __half2* h = reinterpret_cast<const __half2*>(&u);
@@ -67,6 +74,13 @@ template <> struct Half8<__nv_bfloat16> {
       f[2 * i] = t.x;
       f[2 * i + 1] = t.y;
     }
+  }
+  __device__ static __forceinline__ uint4 from_float(const float (&f)[8]) {
+    uint4 u;
+    __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + 1]);
+    return u;
   }
   __device__ static __forceinline__ float absmax(const uint4& u) {
     const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
