@@ -145,9 +145,63 @@ int scale_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows) {
                    CU_TENSOR_MAP_SWIZZLE_NONE);
 }
 
+// Workspace of the chunk kernel: partial sums as above with 256 rows per item, and the schedule.
+struct ChunkWs {
+  size_t ml, desc, items, prefix, pieces, per, bytes;  // offsets; the partial sums come first
+};
+ChunkWs chunk_ws(int64_t D, int64_t max_items) {
+  const size_t rows = size_t(2) * sage::kChunkPieces * sage::kChunkRows;
+  ChunkWs w;
+  w.ml = align256(rows * D * 4);
+  w.desc = w.ml + align256(rows * 4 * 4);
+  w.items = w.desc + align256(sizeof(int4) * sage::kChunkPieces);
+  w.prefix = w.items + align256(sizeof(sage::ChunkItem) * max_items);
+  w.pieces = w.prefix + align256(sizeof(int64_t) * max_items);
+  w.per = w.pieces + align256(sizeof(sage::ChunkPiece) * sage::kChunkPieces);
+  w.bytes = w.per + 256;
+  return w;
+}
+// Blocks of query rows of a call: a sequence's last block may be partly filled.
+int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q * G / sage::kChunkRows + batch; }
+
+// Which kernel: an item of 16 query rows per key/value head streams the cache once per item, so a
+// sequence of more rows reads it several times; from there on the tensor-core tiles of 256 rows win.
+bool chunk_route(int64_t max_seqlen_q, int64_t G, bool i8) { return !i8 && max_seqlen_q * G > sage::kDecRows; }
+
 struct PagedMaps {
   CUtensorMap k, v, ks, vs;
 };
+
+// A launch that may start while its predecessor in the stream still runs; the kernel waits for it on
+// the device (griddepcontrol.wait) before it reads anything the predecessor writes.
+template <typename... A>
+int launch_early(void (*kern)(A...), dim3 grid, int threads, int smem, cudaStream_t st, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  SAGE_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, args...));
+  return SAGE_OK;
+}
+
+template <int D, typename T>
+int launch_chunk(const PagedMaps& m, const sage::ChunkParams& p, int max_rows, cudaStream_t st) {
+  using C = sage::ChunkCfg<D, T>;
+  auto kern = sage::paged_chunk_kernel<D, T>;
+  if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES)) return rc;
+  sage::paged_schedule_kernel<<<1, sage::kScheduleThreads, 0, st>>>(p);
+  SAGE_CUDA_TRY(cudaGetLastError());
+  if (int rc = launch_early(kern, dim3(sage::kChunkPieces), sage::kChunkThreads, C::SMEM_BYTES, st, m.k, m.v, p)) return rc;
+  const unsigned groups = (unsigned)cdiv(std::min(max_rows, sage::kChunkRows), sage::kCombineThreads / 32);
+  return launch_early(sage::paged_combine_kernel<D, false, T, sage::kChunkRows, 1>, dim3(sage::kChunkPieces, groups),
+                      sage::kCombineThreads, 0, st, p.d);
+}
 
 template <int D, bool I8, typename T>
 int launch_decode(const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
@@ -156,18 +210,8 @@ int launch_decode(const PagedMaps& m, const sage::DecodeParams& p, int max_rows,
   if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
   kern<<<sage::kDecPieces, sage::kDecThreads, C::SMEM, st>>>(m.k, m.v, m.ks, m.vs, p);
   SAGE_CUDA_TRY(cudaGetLastError());
-  // the join starts while the pieces run and waits on the device for all of them
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(sage::kDecPieces, (unsigned)std::min(max_rows, sage::kDecRows));
-  cfg.blockDim = dim3(sage::kCombineThreads);
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  SAGE_CUDA_TRY(cudaLaunchKernelEx(&cfg, sage::paged_combine_kernel<D, I8, T>, p));
-  return SAGE_OK;
+  return launch_early(sage::paged_combine_kernel<D, I8, T, sage::kDecRows, 8>,
+                      dim3(sage::kDecPieces, (unsigned)std::min(max_rows, sage::kDecRows)), sage::kCombineThreads, 0, st, p);
 }
 
 template <int D>
@@ -203,6 +247,10 @@ int sage_paged_gather(const sage_paged_cache* cache, void* k, void* v, const int
 size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q, int64_t batch, int64_t total_q,
                                   int64_t max_seqlen_q, int64_t pages_per_seq) {
   if (!cache || heads_q <= 0 || batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || pages_per_seq <= 0) return 0;
+  if (cache->heads_kv <= 0 || heads_q % cache->heads_kv) return 0;
+  const int64_t G = heads_q / cache->heads_kv;
+  if (chunk_route(max_seqlen_q, G, cache->storage == SAGE_CACHE_INT8))
+    return chunk_ws(cache->head_dim, chunk_items(batch, total_q, G)).bytes;
   return decode_ws_bytes(cache->head_dim);
 }
 
@@ -245,15 +293,6 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   if (int rc = check_arch()) return rc;
   const bool i8 = c->storage == SAGE_CACHE_INT8, bf = c->dtype == SAGE_DTYPE_BF16;
   const int64_t D = c->head_dim;
-  PagedMaps m;
-  if (int rc = cache_map(&m.k, c, false, sage::kDecKeys)) return rc;
-  if (int rc = cache_map(&m.v, c, true, sage::kDecKeys)) return rc;
-  m.ks = m.k;
-  m.vs = m.v;
-  if (i8) {
-    if (int rc = scale_map(&m.ks, c, false, sage::kDecKeys)) return rc;
-    if (int rc = scale_map(&m.vs, c, true, sage::kDecKeys)) return rc;
-  }
   p.q = q; p.o = o;
   p.q_sh = q_strides[0]; p.q_st = q_strides[1]; p.o_sh = o_strides[0]; p.o_st = o_strides[1];
   p.Hkv = (int)c->heads_kv; p.G = (int)G;
@@ -263,14 +302,40 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   p.sinks = (int)std::min<int64_t>(sinks, 1LL << 30);
   const double s = sm_scale > 0.0f ? static_cast<double>(sm_scale) : 1.0 / std::sqrt(static_cast<double>(D));
   p.scale_log2 = static_cast<float>(s * 1.4426950408889634);
-  char* w = static_cast<char*>(workspace);
-  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
-  p.part = reinterpret_cast<float*>(w);
-  p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
-  p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
   p.wait_limit_ns = wait_limit_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, 1 << 20);
+  char* w = static_cast<char*>(workspace);
+  p.part = reinterpret_cast<float*>(w);
+  const bool chunk = chunk_route(max_seqlen_q, G, i8);
+  const int tile = chunk ? 128 : sage::kDecKeys;  // keys of a tile
+  PagedMaps m;
+  if (int rc = cache_map(&m.k, c, false, tile)) return rc;
+  if (int rc = cache_map(&m.v, c, true, tile)) return rc;
+  if (chunk) {
+    sage::ChunkParams cp{};
+    const int64_t items = chunk_items(batch, total_q, G);
+    const ChunkWs o = chunk_ws(D, items);
+    p.part_ml = reinterpret_cast<float*>(w + o.ml);
+    p.desc = reinterpret_cast<int4*>(w + o.desc);
+    cp.d = p;
+    cp.items = reinterpret_cast<sage::ChunkItem*>(w + o.items);
+    cp.prefix = reinterpret_cast<int64_t*>(w + o.prefix);
+    cp.pieces = reinterpret_cast<sage::ChunkPiece*>(w + o.pieces);
+    cp.per = reinterpret_cast<int*>(w + o.per);
+    cp.max_items = (int)items;
+    if (D == 128) return bf ? launch_chunk<128, __nv_bfloat16>(m, cp, max_rows, st) : launch_chunk<128, __half>(m, cp, max_rows, st);
+    return bf ? launch_chunk<64, __nv_bfloat16>(m, cp, max_rows, st) : launch_chunk<64, __half>(m, cp, max_rows, st);
+  }
+  m.ks = m.k;
+  m.vs = m.v;
+  if (i8) {
+    if (int rc = scale_map(&m.ks, c, false, tile)) return rc;
+    if (int rc = scale_map(&m.vs, c, true, tile)) return rc;
+  }
+  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
+  p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
+  p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
   return D == 128 ? decode_dispatch<128>(i8, bf, m, p, max_rows, st) : decode_dispatch<64>(i8, bf, m, p, max_rows, st);
 }
 

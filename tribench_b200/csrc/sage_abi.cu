@@ -17,6 +17,7 @@
 
 #include "../../include/sage_sm100.h"
 #include "sage_attn.cuh"
+#include "sage_chunk.cuh"
 #include "sage_decode.cuh"
 #include "sage_paged.cuh"
 #include "sage_quant.cuh"
