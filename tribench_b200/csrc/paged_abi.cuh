@@ -73,6 +73,15 @@ Span scale_span(const sage_paged_cache* c, bool v) {
   return buffer_span(v ? c->v_scale : c->k_scale, static_cast<size_t>(c->num_pages * c->heads_kv * c->page_size) * 4);
 }
 
+sage::PagedStore paged_store(const sage_paged_cache* c) {
+  sage::PagedStore s{};
+  s.k = c->k; s.v = c->v; s.k_scale = c->k_scale; s.v_scale = c->v_scale; s.k_mean = c->k_mean;
+  s.k_sp = c->k_strides[0]; s.k_sh = c->k_strides[1]; s.k_st = c->k_strides[2];
+  s.v_sp = c->v_strides[0]; s.v_sh = c->v_strides[1]; s.v_st = c->v_strides[2];
+  s.pages = (int)c->num_pages; s.page_shift = page_shift(c); s.heads = (int)c->heads_kv;
+  return s;
+}
+
 template <bool READ>
 int paged_move(const sage_paged_cache* c, const void* k, const void* v, const int64_t* ks, const int64_t* vs,
                const int32_t* table, int64_t table_stride, int64_t width, const int32_t* lens, const int32_t* cu,
@@ -95,10 +104,7 @@ int paged_move(const sage_paged_cache* c, const void* k, const void* v, const in
       return fail(SAGE_ERR_INVALID_ARG, "k or v overlaps the cache");
   if (READ && spans_overlap(sk, sv)) return fail(SAGE_ERR_INVALID_ARG, "k and v overlap each other");
   if (int rc = check_arch()) return rc;
-  p.c.k = c->k; p.c.v = c->v; p.c.k_scale = c->k_scale; p.c.v_scale = c->v_scale; p.c.k_mean = c->k_mean;
-  p.c.k_sp = c->k_strides[0]; p.c.k_sh = c->k_strides[1]; p.c.k_st = c->k_strides[2];
-  p.c.v_sp = c->v_strides[0]; p.c.v_sh = c->v_strides[1]; p.c.v_st = c->v_strides[2];
-  p.c.pages = (int)c->num_pages; p.c.page_shift = page_shift(c); p.c.heads = (int)c->heads_kv;
+  p.c = paged_store(c);
   p.k = const_cast<void*>(k); p.v = const_cast<void*>(v);
   p.k_sh = ks[0]; p.k_st = ks[1]; p.v_sh = vs[0]; p.v_st = vs[1];
   const unsigned grid = (unsigned)cdiv(tokens, sage::kPagedThreads / 32);
@@ -147,7 +153,7 @@ int scale_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows) {
 
 // Workspace of the chunk kernel: partial sums as above with 256 rows per item, and the schedule.
 struct ChunkWs {
-  size_t ml, desc, items, prefix, pieces, per, bytes;  // offsets; the partial sums come first
+  size_t ml, desc, items, prefix, pieces, bytes;  // offsets; the partial sums come first
 };
 ChunkWs chunk_ws(int64_t D, int64_t max_items) {
   const size_t rows = size_t(2) * sage::kChunkPieces * sage::kChunkRows;
@@ -157,19 +163,40 @@ ChunkWs chunk_ws(int64_t D, int64_t max_items) {
   w.items = w.desc + align256(sizeof(int4) * sage::kChunkPieces);
   w.prefix = w.items + align256(sizeof(sage::ChunkItem) * max_items);
   w.pieces = w.prefix + align256(sizeof(int64_t) * max_items);
-  w.per = w.pieces + align256(sizeof(sage::ChunkPiece) * sage::kChunkPieces);
-  w.bytes = w.per + 256;
+  w.bytes = w.pieces + align256(sizeof(sage::ChunkPiece) * sage::kChunkPieces);
   return w;
 }
+// Rows of a query tile: G heads in `parts` equal parts of at most 128, TT tokens.
+struct ChunkTile {
+  int64_t parts, Gp, TT;
+};
+ChunkTile chunk_tile(int64_t G) {
+  const int64_t parts = cdiv(G, 128), Gp = cdiv(G, parts);
+  return {parts, Gp, 128 / Gp};
+}
 // Blocks of query rows of a call: a sequence's last block may be partly filled.
-int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q * G / sage::kChunkRows + batch; }
+int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q / (2 * chunk_tile(G).TT) + batch; }
 
 // Which kernel: an item of 16 query rows per key/value head streams the cache once per item, so a
 // sequence of more rows reads it several times; from there on the tensor-core tiles of 256 rows win.
-bool chunk_route(int64_t max_seqlen_q, int64_t G, bool i8) { return !i8 && max_seqlen_q * G > sage::kDecRows; }
+bool chunk_route(int64_t max_seqlen_q, int64_t G) { return max_seqlen_q * G > sage::kDecRows; }
+
+// Tensor map of the packed queries: boxes of Gp heads by TT tokens by 64 channels.
+int query_map(CUtensorMap* map, const void* q, int dtype, int64_t D, int64_t heads, int64_t tokens, int64_t sh, int64_t st,
+              const ChunkTile& t) {
+  cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens};
+  cuuint64_t strides[2] = {(cuuint64_t)(sh * 2), (cuuint64_t)(st * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)t.Gp, (cuuint32_t)t.TT};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = g_encode(map, dtype == SAGE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+                              const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(SAGE_ERR_CUDA, "cuTensorMapEncodeTiled failed (CUresult %d)", (int)r);
+  return SAGE_OK;
+}
 
 struct PagedMaps {
-  CUtensorMap k, v, ks, vs;
+  CUtensorMap q, k, v, ks, vs;
 };
 
 // A launch that may start while its predecessor in the stream still runs; the kernel waits for it on
@@ -190,17 +217,17 @@ int launch_early(void (*kern)(A...), dim3 grid, int threads, int smem, cudaStrea
   return SAGE_OK;
 }
 
-template <int D, typename T>
-int launch_chunk(const PagedMaps& m, const sage::ChunkParams& p, int max_rows, cudaStream_t st) {
-  using C = sage::ChunkCfg<D, T>;
-  auto kern = sage::paged_chunk_kernel<D, T>;
+template <int D, bool I8, typename T>
+int launch_chunk(const PagedMaps& m, const sage::ChunkParams& p, cudaStream_t st) {
+  using C = sage::ChunkCfg<D, I8, T>;
+  auto kern = sage::paged_chunk_kernel<D, I8, T>;
   if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM_BYTES)) return rc;
   sage::paged_schedule_kernel<<<1, sage::kScheduleThreads, 0, st>>>(p);
   SAGE_CUDA_TRY(cudaGetLastError());
-  if (int rc = launch_early(kern, dim3(sage::kChunkPieces), sage::kChunkThreads, C::SMEM_BYTES, st, m.k, m.v, p)) return rc;
-  const unsigned groups = (unsigned)cdiv(std::min(max_rows, sage::kChunkRows), sage::kCombineThreads / 32);
-  return launch_early(sage::paged_combine_kernel<D, false, T, sage::kChunkRows, 1>, dim3(sage::kChunkPieces, groups),
-                      sage::kCombineThreads, 0, st, p.d);
+  if (int rc = launch_early(kern, dim3(sage::kChunkPieces), sage::kChunkThreads, C::SMEM_BYTES, st, m.q, m.k, m.v, p)) return rc;
+  const int64_t rows = p.d.s.max_new >= p.d.TT ? sage::kChunkRows : p.d.s.max_new * p.d.Gp;  // of a block, at most
+  return launch_early(sage::paged_chunk_join_kernel<D, I8, T>, dim3(sage::kChunkPieces, (unsigned)cdiv(rows, sage::kJoinRows)),
+                      sage::kJoinRows * D / 4, 0, st, p.d);
 }
 
 template <int D, bool I8, typename T>
@@ -210,8 +237,14 @@ int launch_decode(const PagedMaps& m, const sage::DecodeParams& p, int max_rows,
   if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
   kern<<<sage::kDecPieces, sage::kDecThreads, C::SMEM, st>>>(m.k, m.v, m.ks, m.vs, p);
   SAGE_CUDA_TRY(cudaGetLastError());
-  return launch_early(sage::paged_combine_kernel<D, I8, T, sage::kDecRows, 8>,
-                      dim3(sage::kDecPieces, (unsigned)std::min(max_rows, sage::kDecRows)), sage::kCombineThreads, 0, st, p);
+  return launch_early(sage::paged_combine_kernel<D, I8, T>,
+                      dim3(sage::kDecPieces, (unsigned)max_rows), sage::kCombineThreads, 0, st, p);
+}
+
+template <int D>
+int chunk_dispatch(bool i8, bool bf, const PagedMaps& m, const sage::ChunkParams& p, cudaStream_t st) {
+  if (i8) return bf ? launch_chunk<D, true, __nv_bfloat16>(m, p, st) : launch_chunk<D, true, __half>(m, p, st);
+  return bf ? launch_chunk<D, false, __nv_bfloat16>(m, p, st) : launch_chunk<D, false, __half>(m, p, st);
 }
 
 template <int D>
@@ -249,7 +282,7 @@ size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q
   if (!cache || heads_q <= 0 || batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || pages_per_seq <= 0) return 0;
   if (cache->heads_kv <= 0 || heads_q % cache->heads_kv) return 0;
   const int64_t G = heads_q / cache->heads_kv;
-  if (chunk_route(max_seqlen_q, G, cache->storage == SAGE_CACHE_INT8))
+  if (chunk_route(max_seqlen_q, G))
     return chunk_ws(cache->head_dim, chunk_items(batch, total_q, G)).bytes;
   return decode_ws_bytes(cache->head_dim);
 }
@@ -304,10 +337,9 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   p.scale_log2 = static_cast<float>(s * 1.4426950408889634);
   p.wait_limit_ns = wait_limit_ns();
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, 1 << 20);
   char* w = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(w);
-  const bool chunk = chunk_route(max_seqlen_q, G, i8);
+  const bool chunk = chunk_route(max_seqlen_q, G);
   const int tile = chunk ? 128 : sage::kDecKeys;  // keys of a tile
   PagedMaps m;
   if (int rc = cache_map(&m.k, c, false, tile)) return rc;
@@ -316,19 +348,22 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
     sage::ChunkParams cp{};
     const int64_t items = chunk_items(batch, total_q, G);
     const ChunkWs o = chunk_ws(D, items);
+    const ChunkTile t = chunk_tile(G);
+    if (int rc = query_map(&m.q, q, c->dtype, D, heads_q, total_q, q_strides[0], q_strides[1], t)) return rc;
+    p.parts = (int)t.parts; p.Gp = (int)t.Gp; p.TT = (int)t.TT;
     p.part_ml = reinterpret_cast<float*>(w + o.ml);
     p.desc = reinterpret_cast<int4*>(w + o.desc);
     cp.d = p;
     cp.items = reinterpret_cast<sage::ChunkItem*>(w + o.items);
     cp.prefix = reinterpret_cast<int64_t*>(w + o.prefix);
     cp.pieces = reinterpret_cast<sage::ChunkPiece*>(w + o.pieces);
-    cp.per = reinterpret_cast<int*>(w + o.per);
     cp.max_items = (int)items;
-    if (D == 128) return bf ? launch_chunk<128, __nv_bfloat16>(m, cp, max_rows, st) : launch_chunk<128, __half>(m, cp, max_rows, st);
-    return bf ? launch_chunk<64, __nv_bfloat16>(m, cp, max_rows, st) : launch_chunk<64, __half>(m, cp, max_rows, st);
+    if (i8) cp.c = paged_store(c);
+    return D == 128 ? chunk_dispatch<128>(i8, bf, m, cp, st) : chunk_dispatch<64>(i8, bf, m, cp, st);
   }
   m.ks = m.k;
   m.vs = m.v;
+  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, sage::kDecRows);
   if (i8) {
     if (int rc = scale_map(&m.ks, c, false, tile)) return rc;
     if (int rc = scale_map(&m.vs, c, true, tile)) return rc;

@@ -6,9 +6,11 @@
 // pipeline this is: two 128-row query tiles, S = Q K^T and O += P V as tcgen05.mma into TMEM, one
 // softmax warpgroup per query tile, MMA issued by one thread.
 //
-// Rows. The rows of one key/value head are the (token, query head of the group) pairs in that order:
-// row r of a sequence is token r / G, head r % G. A block of 256 rows then covers 256 / G tokens, all
-// query heads of the group sharing every tile of keys, and a short chunk of G heads still fills rows.
+// Rows. A query tile holds TT = 128 / G tokens times the G query heads of the group (row = token * G +
+// head; a few rows stay unused where G does not divide 128), so that all query heads of the group share
+// every tile of keys and a short chunk still fills rows. One TMA box of G heads by TT tokens per
+// 64 channels is a query tile. A group of more than 128 heads is cut into equal parts, each treated as
+// a key/value head of its own. A block is two query tiles.
 //
 // Work split. Blocks of one sequence need different numbers of key tiles (causal mask, window). A
 // one-block kernel (paged_schedule_kernel) lists the blocks with their tiles and cuts the line of all
@@ -16,9 +18,16 @@
 // segment by segment, the tile ring running on across segments. A block cut between pieces leaves
 // fp32 partial sums, joined afterwards in a fixed order, as in sage_decode.cuh.
 //
-// Warps: 0-7 softmax (two warpgroups), 8 TMA producer, 9 MMA issuer, 10-11 helpers, which bring the
-// next segment's query rows in with cp.async as soon as its last Q K^T has run, and put zeros over rows
-// of V that no query sees (an unused row may hold a NaN, which its weight of 0 would not silence).
+// INT8 cache: helper warps turn the codes into fp16 tiles (exact) in shared memory, in the layout the
+// TMA load would give, and the scales stay out of the products: scores are multiplied by k_scale per
+// column in fp32, P by v_scale before it is rounded to fp16, in units of a power of two 2^E that
+// follows the largest v_scale of the segment (E is raised, and O rescaled, once a tile exceeds it by
+// 2^4; P < 2^8 * 2^5 stays inside fp16). bf16 queries are brought to fp16 by a power of two per row.
+//
+// Warps: 0-7 softmax (two warpgroups), 8 TMA producer of K and V, 9 MMA issuer, 10 loads the next
+// segment's queries as soon as the last Q K^T of this one has run, 11 puts zeros over rows of V that no
+// query sees (an unused row may hold a NaN, which its weight of 0 would not silence). INT8: 8 loads
+// queries and scales, 10 converts K, 11 converts V.
 #pragma once
 
 #include "sage_attn.cuh"
@@ -26,7 +35,7 @@
 
 namespace sage {
 
-constexpr int kChunkRows = 256;     // query rows per block
+constexpr int kChunkRows = 256;     // query rows per block, the unused ones included
 constexpr int kChunkPieces = 148;   // CTAs: one per SM
 constexpr int kChunkThreads = 384;
 
@@ -36,20 +45,26 @@ struct ChunkItem {
   int blk, ns, tw, count;
 };
 struct ChunkPiece {
-  int item, head, tile, count;  // where it starts, tiles
+  int item, head, tile;                 // where it starts
+  int last_item, last_head, last_tile;  // where the next piece starts
+  int count, pad;                       // 0: empty
 };
+// What a block costs beyond its tiles (queries in, output out, an empty pipeline), in tiles: without
+// it, pieces with many short blocks end long after the others (the first rows of a causal prompt).
+constexpr int kChunkSetup = 2;
 
 struct ChunkParams {
   DecodeParams d;
   ChunkItem* items;
-  int64_t* prefix;      // [items + 1] tiles of one head before an item (schedule only)
+  int64_t* prefix;      // [items] line length of one head before an item (schedule only)
   ChunkPiece* pieces;   // [kChunkPieces]
-  int* per;             // tiles of a piece
   int max_items;
+  PagedStore c;         // INT8 only
 };
 
-template <int D, typename T>
+template <int D, bool I8, typename T>
 struct ChunkCfg {
+  using M = typename std::conditional<I8, __half, T>::type;  // operand type of the products
   static constexpr bool PRE_BIAS = false, QK_F16 = true, PV_FP8 = false;
   static constexpr int BM = 128, BN = 128;
   static constexpr int NS = (D == 128) ? 2 : 4;  // K/V ring stages
@@ -57,10 +72,17 @@ struct ChunkCfg {
   static constexpr int OFF_Q = 0;
   static constexpr int OFF_K = OFF_Q + 2 * TILE;
   static constexpr int OFF_V = OFF_K + NS * TILE;
-  static constexpr int OFF_BAR = OFF_V + NS * TILE;
-  static constexpr int NUM_BARS = 2 + 4 * NS + 12;
+  static constexpr int OUT_CH = (I8 && D == 128) ? 32 : 64;  // output channels staged at a time
+  static constexpr int OUT_BYTES = 32 * OUT_CH * 2;          // per softmax warp: 32 rows of them
+  static constexpr int OFF_OUT = OFF_V + NS * TILE;
+  static constexpr int OFF_BAR = OFF_OUT + 8 * OUT_BYTES;
+  static constexpr int NUM_BARS = 3 + 6 * NS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int SMEM_BYTES = 1024 + OFF_MISC + 64;
+  static constexpr int OFF_WALK = (OFF_MISC + 8 + 15) / 16 * 16;  // where each softmax warp is in the piece
+  static constexpr int WALK_BYTES = 96;
+  static constexpr int OFF_SCALE = (OFF_WALK + 8 * WALK_BYTES + 15) / 16 * 16;  // INT8: per stage k_scale, v_scale 2^-E
+  static constexpr int OFF_EXP = OFF_SCALE + (I8 ? NS * 1024 : 0);               // and E
+  static constexpr int SMEM_BYTES = 1024 + OFF_EXP + (I8 ? 16 : 0);
   static_assert(SMEM_BYTES <= 227 * 1024 && SMEM_BYTES > 114 * 1024, "one CTA per SM");
   static constexpr int REGS_SOFTMAX = 216, REGS_OTHER = 72;  // as in AttnCfg
   static constexpr uint32_t QK_LAYOUT = kLayoutSW128, QK_SBO = 1024;
@@ -72,7 +94,7 @@ struct ChunkCfg {
   static constexpr uint32_t V_LBO = BN * 128, V_SBO = 1024;
   static constexpr bool SEP_P = (D == 64);
   static constexpr uint32_t P_COL = SEP_P ? 128 + D : 64;
-  static constexpr uint32_t FMT = std::is_same<T, __half>::value ? kFmtF16 : kFmtBF16;
+  static constexpr uint32_t FMT = std::is_same<M, __half>::value ? kFmtF16 : kFmtBF16;
   static constexpr uint32_t IDESC_QK = make_idesc(kFmtD_F32, FMT, FMT, 0, 0, BM, BN);
   static constexpr uint32_t IDESC_PV = make_idesc(kFmtD_F32, FMT, FMT, 0, 1, BM, D);
   static constexpr float LAZY = 8.0f;
@@ -80,15 +102,14 @@ struct ChunkCfg {
 };
 
 // ------------------------------------------------------------------ schedule
-__device__ __forceinline__ int chunk_blocks(const PagedSeq& sq, int G) {
-  return (sq.n * G + kChunkRows - 1) / kChunkRows;
+__device__ __forceinline__ int chunk_blocks(const ChunkParams& p, const PagedSeq& sq) {
+  return (sq.n + 2 * p.d.TT - 1) / (2 * p.d.TT);
 }
 
 // The tiles of 128 keys that block `blk` of a sequence needs.
 __device__ __forceinline__ void chunk_tiles(const ChunkParams& p, const PagedSeq& sq, int blk, ChunkItem* it) {
-  const int G = p.d.G;
-  const int tok_a = blk * kChunkRows / G, tok_b = min(sq.n * G, (blk + 1) * kChunkRows) - 1;
-  const int last = tok_b / G, first = sq.len - sq.n;
+  const int tok_a = blk * 2 * p.d.TT, last = min(sq.n, tok_a + 2 * p.d.TT) - 1;
+  const int first = sq.len - sq.n;
   const int lo = p.d.window ? max(0, first + tok_a - p.d.window + 1) : 0;
   const int hi = p.d.causal ? first + last + 1 : sq.len;
   it->ns = p.d.window ? min((min(p.d.sinks, lo) + 127) / 128, (max(hi, 0) + 127) / 128) : 0;
@@ -96,9 +117,12 @@ __device__ __forceinline__ void chunk_tiles(const ChunkParams& p, const PagedSeq
   it->count = max(1, it->ns + max(0, (hi + 127) / 128 - it->tw));
 }
 
-constexpr int kScheduleThreads = 1024;
+constexpr int kScheduleThreads = 512;
+constexpr int kSchedulePrefix = 2048;  // blocks whose line positions stay in shared memory
 __global__ void __launch_bounds__(kScheduleThreads) paged_schedule_kernel(const ChunkParams p) {
-  __shared__ int64_t s_warp[32];
+  __shared__ int64_t s_warp[kScheduleThreads / 32];
+  __shared__ int64_t s_prefix[kSchedulePrefix];
+  __shared__ int s_count[kSchedulePrefix];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   auto block_scan = [&](int64_t v, int64_t* total) {  // exclusive prefix over the block
@@ -111,7 +135,7 @@ __global__ void __launch_bounds__(kScheduleThreads) paged_schedule_kernel(const 
     __syncthreads();
     if (lane == 31) s_warp[warp] = x;
     __syncthreads();
-    int64_t w = s_warp[lane];
+    int64_t w = lane < kScheduleThreads / 32 ? s_warp[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t up = __shfl_up_sync(0xffffffffu, w, o);
@@ -127,16 +151,17 @@ __global__ void __launch_bounds__(kScheduleThreads) paged_schedule_kernel(const 
     const int b = b0 + tid;
     PagedSeq sq{0, 0, 0};
     if (b < p.d.s.batch) sq = paged_seq(p.d.s, b);
-    const int nb = chunk_blocks(sq, p.d.G);
+    const int nb = chunk_blocks(p, sq);
     int64_t total = 0;
     const int64_t at = n_items + block_scan(nb, &total);
-    for (int l = 0; l < 32; ++l) {
+    for (unsigned todo = __ballot_sync(0xffffffffu, nb > 0); todo; todo &= todo - 1) {
+      const int l = __ffs(todo) - 1;
       PagedSeq q;
       q.base = __shfl_sync(0xffffffffu, sq.base, l);
       q.n = __shfl_sync(0xffffffffu, sq.n, l);
       q.len = __shfl_sync(0xffffffffu, sq.len, l);
       const int64_t off = __shfl_sync(0xffffffffu, at, l);
-      const int blocks = chunk_blocks(q, p.d.G);
+      const int blocks = __shfl_sync(0xffffffffu, nb, l);
       for (int k = lane; k < blocks; k += 32) {
         if (off + k >= p.max_items) break;  // the host's bound holds for any prefix sums; kept as a fence
         ChunkItem it;
@@ -144,96 +169,147 @@ __global__ void __launch_bounds__(kScheduleThreads) paged_schedule_kernel(const 
         it.blk = k;
         chunk_tiles(p, q, k, &it);
         p.items[off + k] = it;
+        if (off + k < kSchedulePrefix) s_count[off + k] = it.count + kChunkSetup;
       }
     }
     n_items += total;
   }
   if (n_items > p.max_items) n_items = p.max_items;
   __syncthreads();
-  // ---- tiles before each block
-  int64_t tiles = 0;
+  // ---- the line: a block takes its tiles and kChunkSetup units before them, for every head
+  const int heads = p.d.Hkv * p.d.parts;
+  int64_t line = 0;
   for (int64_t i0 = 0; i0 < n_items; i0 += kScheduleThreads) {
     const int64_t i = i0 + tid;
+    const int len = i >= n_items ? 0 : i < kSchedulePrefix ? s_count[i] : p.items[i].count + kChunkSetup;
     int64_t total = 0;
-    const int64_t at = tiles + block_scan(i < n_items ? p.items[i].count : 0, &total);
-    if (i < n_items) p.prefix[i] = at;
-    tiles += total;
+    const int64_t at = (line + block_scan(len, &total)) * heads;
+    if (i < n_items) {
+      if (i < kSchedulePrefix) s_prefix[i] = at;
+      else p.prefix[i] = at;
+    }
+    line += total;
   }
   __syncthreads();
-  // ---- equal pieces of the line
-  const int64_t all = tiles * p.d.Hkv;
+  // ---- equal pieces of it
+  if (tid >= kChunkPieces) return;
+  const int64_t all = line * heads;
   const int64_t per = max((all + kChunkPieces - 1) / kChunkPieces, (int64_t)1);
-  if (tid == 0) *p.per = (int)per;
-  if (tid < kChunkPieces) {
-    ChunkPiece c{0, 0, 0, 0};
-    const int64_t begin = per * tid;
-    if (begin < all) {
-      // the last block whose line position is <= begin
-      int64_t lo = 0, n = n_items;
-      while (n > 1) {
-        const int64_t half = n / 2;
-        if (p.prefix[lo + half] * p.d.Hkv <= begin) { lo += half; n -= half; }
-        else n = half;
-      }
-      const int64_t rem = begin - p.prefix[lo] * p.d.Hkv;
-      const int cnt = p.items[lo].count;
-      c.item = (int)lo;
-      c.head = (int)(rem / cnt);
-      c.tile = (int)(rem % cnt);
-      c.count = (int)min(per, all - begin);
+  // where a position of the line lies: block, head and tile (0 in the units before the tiles)
+  auto find = [&](int64_t at, int* item, int* head, int* tile, int64_t* end) {
+    int64_t lo = 0, n = n_items;
+    while (n > 1) {
+      const int64_t half = n / 2, mid = lo + half;
+      if ((mid < kSchedulePrefix ? s_prefix[mid] : p.prefix[mid]) <= at) { lo = mid; n -= half; }
+      else n = half;
     }
-    p.pieces[tid] = c;
+    const int64_t begin = lo < kSchedulePrefix ? s_prefix[lo] : p.prefix[lo];
+    const unsigned len = lo < kSchedulePrefix ? s_count[lo] : p.items[lo].count + kChunkSetup;
+    *item = (int)lo;
+    *head = (int)((uint64_t)(at - begin) < (1ull << 32) ? (unsigned)(at - begin) / len : (at - begin) / len);
+    const int64_t left = at - begin - (int64_t)*head * len;
+    *tile = max((int)left - kChunkSetup, 0);
+    *end = at - left + len;  // first position behind this head's part
+  };
+  ChunkPiece c{0, 0, 0, 0};
+  int4 cut = make_int4(0, 0, 0, 0);
+  const int64_t begin = per * tid, stop = min(begin + per, all);
+  if (begin < stop) {
+    int64_t end;
+    find(begin, &c.item, &c.head, &c.tile, &end);
+    c.count = 1;  // not empty; the walk ends at (last_item, last_head, last_tile)
+    if (stop < all) find(stop, &c.last_item, &c.last_head, &c.last_tile, &end);
+    else { c.last_item = (int)n_items; c.last_head = 0; c.last_tile = 0; }
+    // the block that this piece begins and does not end, and how many pieces follow that hold the rest
+    if (c.last_tile > 0 && !(c.last_item == c.item && c.last_head == c.head && c.tile > 0)) {
+      const ChunkItem it = p.items[c.last_item];
+      cut = make_int4(it.b, c.last_head, it.blk, (int)((end - 1) / per) - tid);
+    }
   }
+  p.pieces[tid] = c;
+  p.d.desc[tid] = cut;
 }
 
 // ------------------------------------------------------------------ attention
 // One segment of a CTA's piece: tiles [t0, t0 + n) of a block for one head.
 struct ChunkWalk {
   const ChunkItem* items;
-  int item, head, tile, left, Hkv;
+  int item, head, tile, Hkv;
+  int last_item, last_head, last_tile;
+  bool go;
   ChunkItem it;
   int n;
   __device__ __forceinline__ ChunkWalk(const ChunkParams& p, int cta) {
-    const ChunkPiece c = p.pieces[cta];
+    const int4 a = reinterpret_cast<const int4*>(p.pieces + cta)[0], z = reinterpret_cast<const int4*>(p.pieces + cta)[1];
     items = p.items;
-    item = c.item; head = c.head; tile = c.tile; left = c.count;
-    Hkv = p.d.Hkv;
-    if (left > 0) load();
+    item = a.x; head = a.y; tile = a.z;
+    last_item = a.w; last_head = z.x; last_tile = z.y;
+    Hkv = p.d.Hkv * p.d.parts;
+    go = z.z > 0;
+    if (go) load();
+    settle();
   }
   __device__ __forceinline__ void load() {
     const int4 a = reinterpret_cast<const int4*>(items + item)[0], z = reinterpret_cast<const int4*>(items + item)[1];
     it.base = a.x; it.n = a.y; it.len = a.z; it.b = a.w;
     it.blk = z.x; it.ns = z.y; it.tw = z.z; it.count = z.w;
-    n = min(it.count - tile, left);
   }
-  __device__ __forceinline__ bool more() const { return left > 0; }
+  // tiles of the present segment; the piece's last one may be cut short, or be empty
+  __device__ __forceinline__ void settle() {
+    const bool last = item == last_item && head == last_head;
+    n = (last ? last_tile : it.count) - tile;
+    if (n <= 0) go = false;
+  }
+  __device__ __forceinline__ bool more() const { return go; }
+  __device__ __forceinline__ bool whole() const { return tile == 0 && n == it.count; }
   __device__ __forceinline__ void next() {
-    left -= n;
+    if (item == last_item && head == last_head) { go = false; return; }
     tile = 0;
     if (++head == Hkv) {
       head = 0;
       ++item;
-      if (left > 0) load();
-    } else {
-      n = min(it.count, left);
+      if (item > last_item || (item == last_item && last_head == 0 && last_tile == 0)) { go = false; return; }
+      load();
     }
+    settle();
   }
-  __device__ __forceinline__ int rows(int G) const { return min(kChunkRows, it.n * G - it.blk * kChunkRows); }
+  // tokens [first_tok, first_tok + toks) of the sequence's new ones
+  __device__ __forceinline__ int first_tok(const ChunkParams& p) const { return it.blk * 2 * p.d.TT; }
+  __device__ __forceinline__ int toks(const ChunkParams& p) const { return min(2 * p.d.TT, it.n - it.blk * 2 * p.d.TT); }
   __device__ __forceinline__ int key0(int j) const {  // first key of tile `tile + j`
     const int i = tile + j;
     return (i < it.ns ? i : it.tw + i - it.ns) * 128;
   }
 };
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z)
+      : "memory");
 }
 
-template <int D, typename T>
+// The lowest n bits (n may be anything).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+
+// One 16-byte piece of INT8 codes as 16 fp16 values: 32 bytes, as two 16-byte units.
+__device__ __forceinline__ void codes_to_half16(const uint4& w, uint4& a, uint4& z) {
+  const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u, u = w.z ^ 0x80808080u, v = w.w ^ 0x80808080u;
+  a = make_uint4(biased_to_half2(__byte_perm(x, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(x, 0x64646464u, 0x4342)),
+                 biased_to_half2(__byte_perm(y, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(y, 0x64646464u, 0x4342)));
+  z = make_uint4(biased_to_half2(__byte_perm(u, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(u, 0x64646464u, 0x4342)),
+                 biased_to_half2(__byte_perm(v, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(v, 0x64646464u, 0x4342)));
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+
+template <int D, bool I8, typename T>
 __global__ void __launch_bounds__(kChunkThreads, 1)
-    paged_chunk_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                       const ChunkParams cp) {
-  using C = ChunkCfg<D, T>;
+    paged_chunk_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                       const __grid_constant__ CUtensorMap tmV, const ChunkParams cp) {
+  using C = ChunkCfg<D, I8, T>;
+  using M = typename C::M;
+  constexpr bool Q_CONV = I8 && std::is_same<T, __nv_bfloat16>::value;  // queries from bf16 to fp16
   const DecodeParams& p = cp.d;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -242,26 +318,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* bar_vraw = bar_q + 2;  // [stage]: V landed, rows that no query sees still to be cleared
   uint64_t* bar_kfull = bar_vraw + C::NS;
   uint64_t* bar_vfull = bar_kfull + C::NS;
-  uint64_t* bar_kvempty = bar_vfull + C::NS;
-  uint64_t* bar_sfull = bar_kvempty + C::NS;
+  uint64_t* bar_kempty = bar_vfull + C::NS;  // K's slot is free after Q K^T, V's a softmax later
+  uint64_t* bar_vempty = bar_kempty + C::NS;
+  uint64_t* bar_sfull = bar_vempty + C::NS;
   uint64_t* bar_phalf = bar_sfull + 2;
   uint64_t* bar_pfull = bar_phalf + 2;
   uint64_t* bar_odone = bar_pfull + 2;
   uint64_t* bar_sload = bar_odone + 2;
   uint64_t* bar_pvdone = bar_sload + 2;
+  uint64_t* bar_sc = bar_pvdone + 2;    // [stage] INT8: the tile's scales are in place
+  uint64_t* bar_qraw = bar_sc + C::NS;  // bf16 queries landed, to be converted by the softmax threads
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   const uint32_t warp = warp_id(), lane = lane_id();
   const int cta = blockIdx.x;
 
   if (threadIdx.x == 0) {
-    mbar_init(bar_q, 64);  // the helpers' threads
+    mbar_init(bar_q, Q_CONV ? 256 : 1);
+    mbar_init(bar_qraw, 1);
     mbar_init(bar_qfree, 1);
     for (int s = 0; s < C::NS; ++s) {
       mbar_init(bar_vraw + s, 1);
+      mbar_init(bar_sc + s, 1);
       mbar_init(bar_kfull + s, 1);
       mbar_init(bar_vfull + s, 1);
-      mbar_init(bar_kvempty + s, 1);
+      mbar_init(bar_kempty + s, 1);
+      mbar_init(bar_vempty + s, 1);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(bar_sfull + t, 1);
@@ -278,7 +360,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (warp == 8 && lane == 0) {
+  if (!I8 && warp == 8 && lane == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
@@ -288,36 +370,171 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the schedule is written
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  ChunkWalk w(cp, cta);
-  const int G = p.G;
-
+  if (warp >= 8) {
+    regs_dec<C::REGS_OTHER>();
+    ChunkWalk w(cp, cta);
+    // first key behind those that some query of the segment sees, and first of its window
+  auto seen = [&](int* hi, int* lo) {
+    const int first = w.it.len - w.it.n + w.first_tok(cp);
+    *hi = p.causal ? first + w.toks(cp) : w.it.len;
+    *lo = p.window ? first - p.window + 1 : 0;
+  };
   // a tile that holds rows of V which no query of the block sees
   auto ragged = [&](int key0) {
-    const int first = w.it.len - w.it.n, tok_a = w.it.blk * kChunkRows / G;
-    const int tok_b = (w.it.blk * kChunkRows + w.rows(G) - 1) / G;
-    const int hi = p.causal ? first + tok_b + 1 : w.it.len;
-    const int lo = p.window ? first + tok_a - p.window + 1 : 0;
+    int hi, lo;
+    seen(&hi, &lo);
     return key0 + 128 > hi || (key0 < lo && key0 + 128 > p.sinks);
   };
 
-  if (warp >= 8) {
-    regs_dec<C::REGS_OTHER>();
-    if (warp == 8) {
+    // the segment's queries: one box per query tile and 64 channels
+    auto load_queries = [&] {
+      const int nt = w.toks(cp) > p.TT ? 2 : 1, kvh = w.head / p.parts, part = w.head - kvh * p.parts;
+      uint64_t* bar = Q_CONV ? bar_qraw : bar_q;
+      mbar_arrive_expect_tx(bar, nt * C::ATOMS * 128 * p.TT * p.Gp);
+      for (int t = 0; t < nt; ++t)
+        for (int x = 0; x < C::ATOMS; ++x)
+          tma_load_3d(smem + C::OFF_Q + t * C::TILE + x * (128 * 128), &tmQ, bar, x * 64, kvh * p.G + part * p.Gp,
+                      w.it.base + w.first_tok(cp) + t * p.TT);
+    };
+    const int page = 1 << p.page_shift;
+    const int rows = min(page, 128), ppt = 128 / rows;    // rows of a tile in one page, pages of a tile
+    const int batch_tiles = 32 / ppt;                     // tiles whose page numbers the 32 lanes hold
+    auto page_of = [&](int j) {  // this lane's page of tiles [j, j + batch_tiles) of the segment
+      const int tj = j + (int)lane / ppt;
+      if (tj >= w.n) return -1;
+      const int pg = (w.key0(tj) >> p.page_shift) + (int)lane % ppt;
+      return pg < p.s.width ? p.s.table[(int64_t)w.it.b * p.s.table_stride + pg] : -1;
+    };
+    if (I8 && warp == 8) {
+      // ------------------------------------------------------------ queries and scales
+      const int sh = min(p.page_shift, 7);
+      int it = 0;
+      bool ok = true;
+      for (int seg = 0; w.more() && ok; w.next(), ++seg) {
+        if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        if (lane == 0) load_queries();
+        __syncwarp();
+        const int kvh = w.head / p.parts;
+        int hi, lo, ids = 0, e = -200;
+        seen(&hi, &lo);
+        for (int j = 0; j < w.n; ++j, ++it) {
+          const int s = it % C::NS, key0 = w.key0(j), key = key0 + 4 * lane;
+          if (j % batch_tiles == 0) ids = page_of(j);
+          const int id = __shfl_sync(0xffffffffu, ids, (j % batch_tiles) * ppt + ((4 * lane) >> sh));
+          float k4[4] = {0.f, 0.f, 0.f, 0.f}, v4[4] = {0.f, 0.f, 0.f, 0.f};
+          if (id >= 0 && id < cp.c.pages) {
+            const int64_t at = (((int64_t)id * cp.c.heads + kvh) << p.page_shift) + (key & (page - 1));
+            const float4 a = *reinterpret_cast<const float4*>(cp.c.k_scale + at), z = *reinterpret_cast<const float4*>(cp.c.v_scale + at);
+            k4[0] = a.x; k4[1] = a.y; k4[2] = a.z; k4[3] = a.w;
+            v4[0] = z.x; v4[1] = z.y; v4[2] = z.z; v4[3] = z.w;
+          }
+          float m = 0.0f;
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int kx = key + x;
+            if (!(kx < hi && (kx >= lo || kx < p.sinks))) k4[x] = v4[x] = 0.0f;
+            m = fmaxf(m, v4[x]);
+          }
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+          // exponent of the largest scale (a negative one never arises from the cache's own writes)
+          const int et = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 120);
+          if (e == -200 || et > e + 4) e = et;
+          const float down = pow2(-e);
+          if (it >= C::NS) ok = mbar_wait(bar_vempty + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          float4* dst = reinterpret_cast<float4*>(smem + C::OFF_SCALE + s * 1024);
+          dst[lane] = make_float4(k4[0], k4[1], k4[2], k4[3]);
+          dst[32 + lane] = make_float4(v4[0] * down, v4[1] * down, v4[2] * down, v4[3] * down);
+          if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = e;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_sc + s);
+        }
+      }
+    } else if (I8 && warp >= 10) {
+      // ------------------------------------------------------------ codes to fp16 tiles: K (warp 10), V (warp 11)
+      const bool isv = warp == 11;
+      constexpr int LPR = D / 16, RPI = 32 / LPR;  // lanes per row of codes, rows per iteration
+      constexpr int NG = 128 / (8 * RPI);          // groups of eight iterations per tile
+      const int c = lane % LPR, sub = lane / LPR, sh = min(p.page_shift, 7);
+      const char* base = static_cast<const char*>(isv ? cp.c.v : cp.c.k);
+      const int64_t sp = isv ? cp.c.v_sp : cp.c.k_sp, sr = isv ? cp.c.v_st : cp.c.k_st;
+      uint64_t* bar_full = isv ? bar_vfull : bar_kfull;
+      uint64_t* bar_empty = isv ? bar_vempty : bar_kempty;
+      uint8_t* tiles = smem + (isv ? C::OFF_V : C::OFF_K);
+      // state of the loads, which run one group (and so up to one tile) ahead of the conversion
+      int j = 0, ids = 0, key0 = 0, hi = 0, lo = 0;
+      const char* head_base = base;
+      auto enter = [&](bool segment) {  // the tile j of the present segment
+        if (segment) {
+          seen(&hi, &lo);
+          head_base = base + (int64_t)(w.head / p.parts) * (isv ? cp.c.v_sh : cp.c.k_sh) + c * 16;
+        }
+        if (j % batch_tiles == 0) ids = page_of(j);
+        key0 = w.key0(j);
+      };
+      auto load = [&](int row) {
+        const int id = __shfl_sync(0xffffffffu, ids, (j % batch_tiles) * ppt + (row >> sh));
+        const int key = key0 + row;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (w.more() && id >= 0 && id < cp.c.pages && key < hi && (key >= lo || key < p.sinks))
+          x = ldg_nc_v4(head_base + (int64_t)id * sp + (int64_t)(key & (page - 1)) * sr);
+        return x;
+      };
+      uint4 reg[8];
+      bool more = w.more(), ok = true;
+      if (more) {
+        enter(true);
+#pragma unroll
+        for (int u = 0; u < 8; ++u) reg[u] = load(u * RPI + sub);
+      }
+      for (int it = 0; more && ok; ++it) {
+        const int s = it % C::NS;
+        if (it >= C::NS) ok = mbar_wait(bar_empty + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+#pragma unroll 1
+        for (int g = 0; g < NG; ++g) {
+          if (g == NG - 1) {  // the next loads are the next tile's
+            if (++j == w.n) {
+              w.next();
+              j = 0;
+              more = w.more();
+              if (more) enter(true);
+            } else {
+              enter(false);
+            }
+          }
+          const int next = g == NG - 1 ? 0 : g + 1;
+#pragma unroll
+          for (int u = 0; u < 8; ++u) {
+            const int row = (g * 8 + u) * RPI + sub;
+            uint4 a, z;
+            codes_to_half16(reg[u], a, z);
+            reg[u] = load((next * 8 + u) * RPI + sub);
+            // units 2 c and 2 c + 1 of the row's 16-byte units, 8 per 128-byte atom; the upper atom's
+            // lanes store theirs in the other order, against bank conflicts
+            const bool odd = D == 128 && c >= 4;
+            uint8_t* dst = tiles + s * C::TILE + (c >> 2) * (128 * 128) + row * 128;
+            const int u0 = 2 * (c & 3) + (odd ? 1 : 0), u1 = u0 ^ 1;
+            *reinterpret_cast<uint4*>(dst + ((u0 ^ (row & 7)) << 4)) = odd ? z : a;
+            *reinterpret_cast<uint4*>(dst + ((u1 ^ (row & 7)) << 4)) = odd ? a : z;
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_full + s);
+      }
+    } else if (warp == 8) {
       // ------------------------------------------------------------ TMA producer
-      const int page = 1 << p.page_shift;
-      const int rows = min(page, 128), ppt = 128 / rows;    // rows of a box, pages of a tile
-      const int batch_tiles = 32 / ppt;
-      const int boxes = ppt * C::ATOMS;                      // of K, and of V
+      const int boxes = ppt * C::ATOMS;  // of K, and of V
       int it = 0;
       bool ok = true;
       for (; w.more() && ok; w.next()) {
-        const int* table = p.s.table + (int64_t)w.it.b * p.s.table_stride;
-        auto page_of = [&](int j) {  // this lane's page of tiles [j, j + batch_tiles) of the segment
-          const int tj = j + (int)lane / ppt;
-          if (tj >= w.n) return -1;
-          const int pg = (w.key0(tj) >> p.page_shift) + (int)lane % ppt;
-          return pg < p.s.width ? table[pg] : -1;
-        };
+        const int kvh = w.head / p.parts;
         int next = page_of(0);
         for (int j0 = 0; j0 < w.n && ok; j0 += batch_tiles) {
           const int ids = next;
@@ -325,26 +542,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int j1 = min(w.n, j0 + batch_tiles);
           for (int j = j0; j < j1; ++j, ++it) {
             const int s = it % C::NS;
-            if (it >= C::NS) {
-              ok = mbar_wait(bar_kvempty + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+            const int key0 = w.key0(j), y = key0 & (page - 1);
+            const int sub = lane % ppt, atom = lane / ppt;
+            const int id = __shfl_sync(0xffffffffu, ids, (j - j0) * ppt + sub);
+            const int dst = s * C::TILE + atom * (128 * 128) + sub * rows * 128;
+            uint64_t* vbar = (ragged(key0) ? bar_vraw : bar_vfull) + s;
+#pragma unroll
+            for (int isv = 0; isv < 2; ++isv) {
+              if (ok && it >= C::NS)
+                ok = mbar_wait((isv ? bar_vempty : bar_kempty) + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer,
+                               p.wait_limit_ns);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
+              uint64_t* bar = isv ? vbar : bar_kfull + s;
+              if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+              __syncwarp();
+              if (lane < boxes)
+                tma_load_4d(smem + (isv ? C::OFF_V : C::OFF_K) + dst, isv ? &tmV : &tmK, bar, atom * 64, y, kvh, id);
             }
-            const int key0 = w.key0(j);
-            uint64_t* vbar = (ragged(key0) ? bar_vraw : bar_vfull) + s;
-            if (lane == 0) {
-              mbar_arrive_expect_tx(bar_kfull + s, C::TILE);
-              mbar_arrive_expect_tx(vbar, C::TILE);
-            }
-            __syncwarp();
-            const int y = key0 & (page - 1);
-            for (int x = lane; x < (2 * boxes + 31) / 32 * 32; x += 32) {
-              const int sub = x % ppt, rest = x / ppt, atom = rest % C::ATOMS, isv = rest / C::ATOMS;
-              const int id = __shfl_sync(0xffffffffu, ids, (j - j0) * ppt + sub);
-              if (x < 2 * boxes)
-                tma_load_4d(smem + (isv ? C::OFF_V : C::OFF_K) + s * C::TILE + atom * (128 * 128) + sub * rows * 128,
-                            isv ? &tmV : &tmK, isv ? vbar : bar_kfull + s, atom * 64, y, w.head, id);
-            }
+            if (!ok) break;
           }
         }
       }
@@ -364,7 +580,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         int ct0[2] = {0, 0};   // tiles of each query tile before the segment
         bool ok = true;
         for (; w.more() && ok; w.next(), ++seg) {
-          const int nt = w.rows(G) > 128 ? 2 : 1, n = w.n;
+          const int nt = w.toks(cp) > p.TT ? 2 : 1, n = w.n;
           ok = mbar_wait(bar_q, seg & 1, abort_flag, kDevTimeoutMma, p.wait_limit_ns);
           if (ok) ok = mbar_wait(bar_kfull + it0 % C::NS, (it0 / C::NS) & 1, abort_flag, kDevTimeoutMma, p.wait_limit_ns);
           if (!ok) break;
@@ -375,6 +591,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             issue_qk<C>(tmem_base + 256 * t, q_addr + t * C::TILE, k_addr + (it0 % C::NS) * C::TILE, 0);
             umma_commit(bar_sfull + t);
           }
+          umma_commit(bar_kempty + it0 % C::NS);
           if (n == 1) umma_commit(bar_qfree);
           for (int j = 0; ok && j < n; ++j) {
             const int i = it0 + j, s = i % C::NS, s1 = (i + 1) % C::NS;
@@ -388,7 +605,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               tc_fence_after();
               issue_qk<C>(tmem_base + 256 * t, q_addr + t * C::TILE, k_addr + s1 * C::TILE, 0);
               umma_commit(bar_sfull + t);
-              if (j + 2 == n && t + 1 == nt) umma_commit(bar_qfree);  // the block's queries have been read
+              if (t + 1 == nt) {
+                umma_commit(bar_kempty + s1);
+                if (j + 2 == n) umma_commit(bar_qfree);  // the block's queries have been read
+              }
               return true;
             };
             if constexpr (C::SEP_P) {
@@ -425,42 +645,32 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               if constexpr (C::SEP_P) umma_commit(bar_pvdone + t);
               else if (j + 1 < n) ok = next_qk(t);
             }
-            if (ok) umma_commit(bar_kvempty + s);
+            if (ok) umma_commit(bar_vempty + s);
           }
           it0 += n;
           ct0[0] += n;
           if (nt == 2) ct0[1] += n;
         }
       }
+    } else if (warp == 10) {
+      // ------------------------------------------------------------ queries
+      if (elect_one()) {
+        tma_prefetch_desc(&tmQ);
+        bool ok = true;
+        for (int seg = 0; w.more() && ok; w.next(), ++seg) {
+          if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+          if (!ok) break;
+          load_queries();
+        }
+      }
     } else {
-      // ------------------------------------------------------------ helpers: queries, rows of V nobody sees
-      const int hl = (warp - 10) * 32 + lane;
-      int it = 0, seg = 0;
+      // ------------------------------------------------------------ rows of V that no query sees
+      int it = 0;
       uint32_t raw_phase = 0;  // bit s: phase of bar_vraw[s]
       bool ok = true;
-      for (; w.more() && ok; w.next(), ++seg) {
-        if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        constexpr int PR = D / 8;  // 16-byte pieces per row
-        const int rows = w.rows(G), fr0 = w.it.blk * kChunkRows;
-        const int need = (rows > 128 ? 256 : 128) * PR;
-        const char* q = static_cast<const char*>(p.q);
-        const uint32_t q_addr = smem_u32(smem + C::OFF_Q);
-#pragma unroll 4
-        for (int x = hl; x < need; x += 64) {
-          const int row = x / PR, c = x % PR, r = row & 127;
-          const int fr = fr0 + min(row, rows - 1), tok = fr / G, hd = fr - tok * G;
-          cp_async16(q_addr + (row >> 7) * C::TILE + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4),
-                     q + ((int64_t)(w.it.base + tok) * p.q_st + (int64_t)(w.head * G + hd) * p.q_sh + c * 8) * 2, row < rows);
-        }
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        fence_proxy_async_smem();
-        mbar_arrive(bar_q);
-        const int first = w.it.len - w.it.n, tok_a = fr0 / G, tok_b = (fr0 + rows - 1) / G;
-        const int hi = p.causal ? first + tok_b + 1 : w.it.len;
-        const int lo = p.window ? first + tok_a - p.window + 1 : 0;
-        if (warp == 10) continue;
+      for (; w.more() && ok; w.next()) {
+        int hi, lo;
+        seen(&hi, &lo);
         for (int j = 0; j < w.n && ok; ++j, ++it) {
           const int key0 = w.key0(j), s = it % C::NS;
           if (!ragged(key0)) continue;
@@ -497,26 +707,68 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     const uint32_t lane_base = ((warp % 4) * 32u) << 16;
     const uint32_t s_tmem = tmem_base + lane_base + 256 * t;
     const uint32_t o_tmem = s_tmem + 128;
+    const int row_tok = row_in_tile / p.Gp, row_head = row_in_tile - row_tok * p.Gp;
     int ct = 0, segs = 0;  // tiles and segments of this query tile so far
+    int it0 = 0, qseg = 0;  // tiles and segments of the CTA so far
     bool ok = true;
-    int4 cut = make_int4(0, 0, 0, 0);
-    for (; w.more() && ok; w.next()) {
-      const int rows = w.rows(G);
-      if (w.tile == 0 && w.n < w.it.count) {
-        const int per = *cp.per;
-        cut = make_int4(w.it.b, w.head, w.it.blk, (w.it.count - w.n + per - 1) / per);
+    // The walk through the piece lives in shared memory, one per warp: its fifteen registers beside a
+    // row of 128 scores would spill.
+    static_assert(sizeof(ChunkWalk) <= C::WALK_BYTES, "walk");
+    ChunkWalk& w = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * C::WALK_BYTES);
+    if (lane == 0) w = ChunkWalk(cp, cta);
+    __syncwarp();
+    auto step = [&] {
+      __syncwarp();
+      if (lane == 0) w.next();
+      __syncwarp();
+    };
+    for (; ok && w.more(); step()) {
+      const int first_tok = w.first_tok(cp) + t * p.TT;           // of this query tile
+      const int toks = min(p.TT, w.it.n - first_tok);
+      const int n = w.n, it_seg = it0;
+      it0 += n;
+      float scale = p.scale_log2;
+      if constexpr (Q_CONV) {
+        // this thread's query row from bf16 to fp16 in place, in units of a power of two
+        if (!__all_sync(0xffffffffu, mbar_wait(bar_qraw, qseg++ & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
+        if (toks > 0) {
+          uint8_t* q = smem + C::OFF_Q + t * C::TILE + row_in_tile * 128;
+          uint32_t m = 0;
+          uint4 raw[D / 8];
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            raw[x] = *reinterpret_cast<uint4*>(q + (x >> 3) * (128 * 128) + (((x & 7) ^ (row_in_tile & 7)) << 4));
+            float f[8];
+            Half8<T>::to_float(raw[x], f);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) m = max(m, abs_bits(f[y]));
+          }
+          const int e = min(max((int)(m >> 23) - 127, -126), 126);
+          const float down = pow2(-e);
+          scale *= pow2(e);
+#pragma unroll
+          for (int x = 0; x < D / 8; ++x) {
+            float f[8];
+            Half8<T>::to_float(raw[x], f);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) f[y] *= down;
+            *reinterpret_cast<uint4*>(q + (x >> 3) * (128 * 128) + (((x & 7) ^ (row_in_tile & 7)) << 4)) = Half8<__half>::from_float(f);
+          }
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar_q);
       }
-      if (t * 128 >= rows) continue;  // no rows in this query tile (uniform over the warpgroup)
-      const int n = w.n;
-      const int row = t * 128 + row_in_tile, fr = w.it.blk * kChunkRows + min(row, rows - 1);
-      const int tok = fr / G, hd = fr - tok * G;
-      const int first = w.it.len - w.it.n, pos = first + tok;
-      const int hi = p.causal ? pos + 1 : w.it.len;        // this row sees keys [lo, hi) and those of [0, sinks) below hi
+      if (toks <= 0) continue;  // uniform over the warpgroup
+      const int pos = w.it.len - w.it.n + first_tok + min(row_tok, toks - 1);
+      const int hi = p.causal ? pos + 1 : w.it.len;  // this row sees keys [lo, hi) and those of [0, sinks) below hi
       const int lo = p.window ? pos - p.window + 1 : 0;
       // over the rows of this query tile
-      const int ta = (w.it.blk * kChunkRows + t * 128) / G, tb = (w.it.blk * kChunkRows + min(rows, t * 128 + 128) - 1) / G;
-      const int all_hi = p.causal ? first + ta + 1 : w.it.len, all_lo = p.window ? first + tb - p.window + 1 : 0;
+      const int first = w.it.len - w.it.n + first_tok;
+      const int all_hi = p.causal ? first + 1 : w.it.len, all_lo = p.window ? first + toks - p.window : 0;
       float m_run = -INFINITY, l_run = 0.0f;
+      int e_run = 0;  // INT8: O is in units of 2^e_run
+      int key0 = w.key0(0);
+      const int jump = w.it.ns - 1 - w.tile, jump_to = w.it.tw * 128;  // the tile after tile `jump` lies behind the sinks'
       for (int j = 0; j < n; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar_sfull + t, (ct + j) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
         tc_fence_after();
@@ -531,13 +783,33 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int c = 0; c < 128; ++c) b[c] = __uint_as_float(sr[c]);
         }
-        const int key0 = w.key0(j);
+        float shrink = 1.0f;  // INT8: O's factor where the unit is raised
+        const float4* scales = nullptr;
+        if constexpr (I8) {
+          const int s = (it_seg + j) % C::NS;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_sc + s, ((it_seg + j) / C::NS) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
+          scales = reinterpret_cast<const float4*>(smem + C::OFF_SCALE + s * 1024);
+          const int e = reinterpret_cast<const int*>(smem + C::OFF_EXP)[s];
+          if (j > 0 && e != e_run) shrink = pow2(max(e_run - e, -126));
+          e_run = e;
+#pragma unroll
+          for (int c = 0; c < 128; c += 4) {
+            const float4 ks = scales[c / 4];
+            const float2 x = fmul2(make_float2(b[c], b[c + 1]), make_float2(ks.x, ks.y));
+            const float2 y = fmul2(make_float2(b[c + 2], b[c + 3]), make_float2(ks.z, ks.w));
+            b[c] = x.x; b[c + 1] = x.y; b[c + 2] = y.x; b[c + 3] = y.y;
+          }
+        }
         const int up = hi - key0, down = lo - key0, sk = p.sinks - key0;
         const bool masked = key0 + 128 > all_hi || (key0 < all_lo && key0 + 128 > p.sinks);
+        uint32_t vis[4];  // bit c % 32 of word c / 32: this row sees key c of the tile
         if (masked) {
 #pragma unroll
+          for (int x = 0; x < 4; ++x)
+            vis[x] = low_bits(up - 32 * x) & (~low_bits(down - 32 * x) | low_bits(sk - 32 * x));
+#pragma unroll
           for (int c = 0; c < 128; ++c)
-            if (c >= up || (c < down && c >= sk)) b[c] = -INFINITY;
+            if (!((vis[c / 32] >> (c % 32)) & 1u)) b[c] = -INFINITY;
         }
         float hm[2];
 #pragma unroll
@@ -550,13 +822,13 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           hm[h2] = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmaxf(a[6], a[7]));
         }
-        const float tmax = fmaxf(hm[0], hm[1]) * p.scale_log2;
+        const float tmax = fmaxf(hm[0], hm[1]) * scale;
         const bool upd = tmax > m_run + C::LAZY;
         const float m_new = upd ? tmax : m_run;
         const float alpha = upd ? ex2_approx(m_run - m_new) : 1.0f;
-        const bool rescale = j > 0 && __any_sync(0xffffffffu, upd);
+        const bool rescale = j > 0 && __any_sync(0xffffffffu, upd || (I8 && shrink != 1.0f));
         const float m_use = (m_new == -INFINITY) ? 0.0f : m_new;
-        const float2 scv = make_float2(p.scale_log2, p.scale_log2), ccv = make_float2(-m_use, -m_use);
+        const float2 scv = make_float2(scale, scale), ccv = make_float2(-m_use, -m_use);
         float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) {
@@ -573,15 +845,20 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               e.y = ex2_approx(a.y);
             }
             acc[pr & 3] = fadd2(acc[pr & 3], e);
-            pk[pr] = pack2<T>(e.x, e.y);
+            if constexpr (I8) {
+              const float2 vs = reinterpret_cast<const float2*>(scales + 32)[c / 2];
+              e = fmul2(e, vs);
+            }
+            pk[pr] = pack2<M>(e.x, e.y);
           }
           // the polynomial's least result, 2^-125, is no zero in bf16
-          if (std::is_same<T, __nv_bfloat16>::value && masked) {
+          if (std::is_same<M, __nv_bfloat16>::value && masked) {
 #pragma unroll
             for (int pr = 0; pr < 32; ++pr) {
               const int c = h2 * 64 + 2 * pr;
-              if (c >= up || (c < down && c >= sk)) pk[pr] &= 0xffff0000u;
-              if (c + 1 >= up || (c + 1 < down && c + 1 >= sk)) pk[pr] &= 0xffffu;
+              if ((c % 32) < 32 - C::EMU) continue;
+              const uint32_t v = vis[c / 32] >> (c % 32);
+              pk[pr] &= ((v & 1u) ? 0xffffu : 0u) | ((v & 2u) ? 0xffff0000u : 0u);
             }
           }
           if (h2 == 1) {
@@ -599,7 +876,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               uint32_t orow[32];
               tmem_ld32_sync(o_tmem + c0, orow);
 #pragma unroll
-              for (int c = 0; c < 32; ++c) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * alpha);
+              for (int c = 0; c < 32; ++c) orow[c] = __float_as_uint(__uint_as_float(orow[c]) * (I8 ? alpha * shrink : alpha));
               tmem_st32(o_tmem + c0, orow);
             }
           }
@@ -611,45 +888,116 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         const float2 s01 = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
         l_run = fmaf(l_run, alpha, s01.x + s01.y);
         m_run = m_new;
+        key0 = j == jump ? jump_to : key0 + 128;
       }
       if (!ok) break;
       if (!__all_sync(0xffffffffu, mbar_wait(bar_odone + t, segs & 1, abort_flag, kDevTimeoutEpilogue, p.wait_limit_ns))) { ok = false; break; }
       tc_fence_after();
       ct += n;
       ++segs;
-      const bool whole = w.tile == 0 && n == w.it.count;
-      const float inv = whole ? (m_run == -INFINITY ? 0.0f : 1.0f / l_run) : 1.0f;
+      const bool whole = w.whole();
+      const float inv = m_run == -INFINITY ? 0.0f : (I8 ? pow2(e_run) / l_run : 1.0f / l_run);
       const int64_t slot = 2 * cta + (w.tile == 0 ? 1 : 0);
-      T* dst = static_cast<T*>(p.o) + (int64_t)(w.it.base + tok) * p.o_st + (int64_t)(w.head * G + hd) * p.o_sh;
-      float* part = p.part + (slot * kChunkRows + row) * D;
+      const int kvh = w.head / p.parts, part = w.head - kvh * p.parts, heads = min(p.Gp, p.G - part * p.Gp);
+      const int row = t * 128 + row_in_tile;
+      const bool valid = row_tok < toks && row_head < heads;
+      if (whole) {
+        // Through the warp's part of shared memory, OUT_CH channels at a time: PR consecutive lanes then
+        // store a row's contiguous bytes, where one lane per row would touch 32 lines. Piece c of row r
+        // lies at c ^ swizzle(r), against bank conflicts.
+        constexpr int PR = C::OUT_CH / 8, SW = 8 / PR;  // pieces per row; rows that share 128 bytes
+        uint4* stage = reinterpret_cast<uint4*>(smem + C::OFF_OUT + warp * C::OUT_BYTES);
+        T* out = static_cast<T*>(p.o) + (int64_t)(w.it.base + first_tok) * p.o_st +
+                 (int64_t)(kvh * p.G + part * p.Gp) * p.o_sh;
+        const int piece = lane % PR;
 #pragma unroll
-      for (int c0 = 0; c0 < D; c0 += 32) {
-        uint32_t orow[32];
-        tmem_ld32_sync(o_tmem + c0, orow);
-        if (row < rows) {
-          if (whole) {
+        for (int c0 = 0; c0 < D; c0 += C::OUT_CH) {
+#pragma unroll
+          for (int h2 = 0; h2 < C::OUT_CH / 32; ++h2) {
+            uint32_t orow[32];
+            tmem_ld32_sync(o_tmem + c0 + 32 * h2, orow);
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
               float f[8];
 #pragma unroll
               for (int e = 0; e < 8; ++e) f[e] = __uint_as_float(orow[8 * v + e]) * inv;
-              *reinterpret_cast<uint4*>(dst + c0 + 8 * v) = Half8<T>::from_float(f);
+              stage[lane * PR + ((4 * h2 + v) ^ ((lane / SW) % PR))] = Half8<T>::from_float(f);
             }
-          } else {
+          }
+          __syncwarp();
+#pragma unroll
+          for (int i = 0; i < PR; ++i) {
+            const int r = i * (32 / PR) + lane / PR;
+            const int tok = __shfl_sync(0xffffffffu, row_tok, r), hd = __shfl_sync(0xffffffffu, row_head, r);
+            if (tok < toks && hd < heads)
+              *reinterpret_cast<uint4*>(out + (int64_t)tok * p.o_st + (int64_t)hd * p.o_sh + c0 + piece * 8) =
+                  stage[r * PR + (piece ^ ((r / SW) % PR))];
+          }
+          __syncwarp();
+        }
+      } else {
+        // channels 4 x .. 4 x + 3 of row r at [x][r], so that a warp's store is contiguous
+        float4* dst = reinterpret_cast<float4*>(p.part) + slot * kChunkRows * (D / 4) + row;
+#pragma unroll
+        for (int c0 = 0; c0 < D; c0 += 32) {
+          uint32_t orow[32];
+          tmem_ld32_sync(o_tmem + c0, orow);
+          if (valid) {
 #pragma unroll
             for (int v = 0; v < 8; ++v)
-              *reinterpret_cast<uint4*>(part + c0 + 4 * v) = make_uint4(orow[4 * v], orow[4 * v + 1], orow[4 * v + 2], orow[4 * v + 3]);
+              dst[(c0 / 4 + v) * kChunkRows] =
+                  make_float4(__uint_as_float(orow[4 * v]), __uint_as_float(orow[4 * v + 1]),
+                              __uint_as_float(orow[4 * v + 2]), __uint_as_float(orow[4 * v + 3]));
           }
         }
+        if (valid) *reinterpret_cast<float4*>(p.part_ml + (slot * kChunkRows + row) * 4) = make_float4(m_run, l_run, I8 ? m_run + e_run : m_run, 0.0f);
       }
-      if (!whole && row < rows)
-        *reinterpret_cast<float4*>(p.part_ml + (slot * kChunkRows + row) * 4) = make_float4(m_run, l_run, m_run, 0.0f);
       tc_fence_before();
     }
-    if (threadIdx.x == 0) p.desc[cta] = cut;
     tc_fence_before();
     asm volatile("bar.arrive 2, %0;" ::"n"(kChunkThreads) : "memory");
   }
+}
+
+// Joins the parts of blocks that the pieces' borders cut, as paged_combine_kernel does: eight rows per
+// block, a thread per row and four channels (eight threads read 128 contiguous bytes).
+constexpr int kJoinRows = 8;
+template <int D, bool I8, typename T>
+__global__ void __launch_bounds__(kJoinRows * D / 4) paged_chunk_join_kernel(const DecodeParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 d = p.desc[blockIdx.x];
+  if (d.w == 0) return;
+  const int row = blockIdx.y * kJoinRows + threadIdx.x % kJoinRows, x = threadIdx.x / kJoinRows;
+  const int r = row & 127, rt = r / p.Gp, hd = r - rt * p.Gp;
+  const int kvh = d.y / p.parts, part = d.y - kvh * p.parts;
+  const PagedSeq sq = paged_seq(p.s, d.x);
+  const int tok = (2 * d.z + (row >> 7)) * p.TT + rt;
+  if (rt >= p.TT || tok >= sq.n || part * p.Gp + hd >= p.G) return;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float m = -INFINITY, l = 0.0f, mo = -INFINITY;  // mo: INT8, the outputs' own unit
+#pragma unroll 4
+  for (int j = 0; j <= d.w; ++j) {
+    const int64_t slot = j == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + j);
+    const float4 ml = *reinterpret_cast<const float4*>(p.part_ml + (slot * kChunkRows + row) * 4);
+    const float4 v = reinterpret_cast<const float4*>(p.part)[(slot * (D / 4) + x) * kChunkRows + row];
+    const float mn = fmaxf(m, ml.x), use = mn == -INFINITY ? 0.0f : mn;
+    float a = ex2_approx(m - use), z = ex2_approx(ml.x - use);
+    m = mn;
+    l = fmaf(l, a, ml.y * z);
+    if constexpr (I8) {
+      const float on = fmaxf(mo, ml.z), uo = on == -INFINITY ? 0.0f : on;
+      a = ex2_approx(mo - uo);
+      z = ex2_approx(ml.z - uo);
+      mo = on;
+    }
+    o.x = fmaf(o.x, a, v.x * z);
+    o.y = fmaf(o.y, a, v.y * z);
+    o.z = fmaf(o.z, a, v.z * z);
+    o.w = fmaf(o.w, a, v.w * z);
+  }
+  const float inv = l == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - m) / l : 1.0f / l);
+  T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(kvh * p.G + part * p.Gp + hd) * p.o_sh + x * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }
 
 }  // namespace sage

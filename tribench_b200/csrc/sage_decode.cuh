@@ -52,7 +52,11 @@ struct DecodeParams {
   float scale_log2;                // sm_scale * log2(e)
   float* part;                     // [2 * CTAs][16][D] unnormalised outputs
   float* part_ml;                  // [2 * CTAs][16][4]: max of scores, sum, max of weights
-  int4* desc;                      // [CTAs]: the cut item that ends in a CTA's piece (seq, head, tile, pieces that follow)
+  int4* desc;                      // [CTAs]: the item that a CTA's piece begins and does not end (sequence,
+                                   // head, query tile or block, pieces that follow with its rest; 0: none)
+  // Rows of the chunk kernel's blocks: parts of a head group (1 up to 128 heads), query heads of a
+  // part, tokens of a query tile (128 / Gp)
+  int parts, Gp, TT;
   unsigned long long wait_limit_ns;
 };
 
@@ -635,32 +639,30 @@ __global__ void __launch_bounds__(kDecThreads, 2)
 }
 
 // Joins the pieces of items that the pieces' borders cut: the item that piece c begins without ending
-// (slot 2 c + 1) has its other parts in slots 2 c' of the pieces that follow. A row belongs to WPR
-// warps, which share its parts; lanes hold D / 32 channels each. ROWS: query rows of an item (16: WPR
-// = 8, few rows and often many parts; 256: WPR = 1).
+// (slot 2 c + 1) has its other parts in slots 2 c' of the pieces that follow. Block (c, row) joins one
+// row: eight warps share its parts, lanes hold D / 32 channels each.
 constexpr int kCombineThreads = 256;
-template <int D, bool I8, typename T, int ROWS, int WPR>
+template <int D, bool I8, typename T>
 __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const DecodeParams p) {
-  constexpr int E = D / 32;
-  constexpr int RPB = kCombineThreads / 32 / WPR;  // rows per block
-  __shared__ float s_o[WPR > 1 ? WPR : 1][D];
-  __shared__ float s_ml[WPR > 1 ? WPR : 1][3];
+  constexpr int E = D / 32, W = kCombineThreads / 32;
+  __shared__ float s_o[W][D];
+  __shared__ float s_ml[W][3];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int4 d = p.desc[blockIdx.x];
   if (d.w == 0) return;
-  const int warp = warp_id(), lane = lane_id();
-  const int row = blockIdx.y * RPB + warp / WPR;
+  const int warp = warp_id(), lane = lane_id(), row = blockIdx.y;
   const PagedSeq sq = paged_seq(p.s, d.x);
-  const int fr = d.z * ROWS + row;
-  if (fr >= sq.n * p.G) return;  // WPR = 8: the whole block
+  const int fr = d.z * kDecRows + row;
+  if (fr >= sq.n * p.G) return;
+  const int tok = fr / p.G, hd = fr - tok * p.G;
   float o[E], ms = -INFINITY, l = 0.0f, mo = -INFINITY;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll 4
-  for (int j = warp % WPR; j <= d.w; j += WPR) {
+  for (int j = warp; j <= d.w; j += W) {
     const int64_t slot = j == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + j);
-    const float4 x = *reinterpret_cast<const float4*>(p.part_ml + (slot * ROWS + row) * 4);
-    const float* src = p.part + (slot * ROWS + row) * D + lane * E;
+    const float4 x = *reinterpret_cast<const float4*>(p.part_ml + (slot * kDecRows + row) * 4);
+    const float* src = p.part + (slot * kDecRows + row) * D + lane * E;
     float v[E];
     if constexpr (E == 4) {
       const float4 y = *reinterpret_cast<const float4*>(src);
@@ -678,37 +680,33 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], fa, v[e] * fb);
   }
-  if constexpr (WPR > 1) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
-    if (lane == 0) {
-      s_ml[warp][0] = ms;
-      s_ml[warp][1] = l;
-      s_ml[warp][2] = mo;
-    }
-    __syncthreads();
-    if (warp != 0) return;
-    ms = mo = -INFINITY;
-#pragma unroll
-    for (int w = 0; w < WPR; ++w) {
-      ms = fmaxf(ms, s_ml[w][0]);
-      mo = fmaxf(mo, s_ml[w][2]);
-    }
-    l = 0.0f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) o[e] = 0.0f;
-    const float us = ms == -INFINITY ? 0.0f : ms, uo = mo == -INFINITY ? 0.0f : mo;
-#pragma unroll
-    for (int w = 0; w < WPR; ++w) {
-      l = fmaf(s_ml[w][1], ex2_approx(s_ml[w][0] - us), l);
-      const float f = ex2_approx(s_ml[w][2] - uo);
-#pragma unroll
-      for (int e = 0; e < E; ++e) o[e] = fmaf(s_o[w][lane * E + e], f, o[e]);
-    }
+  for (int e = 0; e < E; ++e) s_o[warp][lane * E + e] = o[e];
+  if (lane == 0) {
+    s_ml[warp][0] = ms;
+    s_ml[warp][1] = l;
+    s_ml[warp][2] = mo;
   }
-  const float us = ms == -INFINITY ? 0.0f : ms;
+  __syncthreads();
+  if (warp != 0) return;
+  ms = mo = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    ms = fmaxf(ms, s_ml[w][0]);
+    mo = fmaxf(mo, s_ml[w][2]);
+  }
+  l = 0.0f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.0f;
+  const float us = ms == -INFINITY ? 0.0f : ms, uo = mo == -INFINITY ? 0.0f : mo;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    l = fmaf(s_ml[w][1], ex2_approx(s_ml[w][0] - us), l);
+    const float f = ex2_approx(s_ml[w][2] - uo);
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = fmaf(s_o[w][lane * E + e], f, o[e]);
+  }
   const float inv = l == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - us) / l : 1.0f / l);
-  const int tok = fr / p.G, hd = fr - tok * p.G;
   T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(d.y * p.G + hd) * p.o_sh + lane * E;
   if constexpr (E == 4)
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));

@@ -22,54 +22,70 @@ every access inside the tensors whatever they hold (see the C header).
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
 from . import _native as N
-from .sage_attn import _DTYPES, _check_tensor, _stream_ptr
+from .sage_attn import _DTYPES, _check_tensor
+
+
+# A step of a small model makes hundreds of these calls, so what runs on the host per call is kept
+# short: stride arrays and workspace sizes are looked up by value, the stream and the current device
+# are asked for directly.
+_strides2 = functools.lru_cache(maxsize=1024)(N.strides2)
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+_HERE = contextlib.nullcontext()
+
+
+def _on(device):
+    """Context with ``device`` current."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _packed2(name: str, t: torch.Tensor, heads: int, dim: int, dtype, device):
     """Checks a packed [tokens, heads, dim] tensor; (tokens, element strides {head, token})."""
-    _check_tensor(name, t, dtype)
-    if t.device != device:
+    if not isinstance(t, torch.Tensor) or t.dtype is not dtype or t.device != device:
+        _check_tensor(name, t, dtype)
         raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != dim:
-        raise ValueError(f"{name} must be a packed [tokens, {heads}, {dim}] tensor, got shape {tuple(t.shape)}")
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != dim:
+        raise ValueError(f"{name} must be a packed [tokens, {heads}, {dim}] tensor, got shape {tuple(shape)}")
     st, sh, sd = t.stride()
     if sd != 1:
         raise ValueError(f"{name}: the head dimension must be contiguous (stride 1)")
     # the stride of an axis of one entry is never used: any valid one serves
-    return t.shape[0], N.strides2(sh if heads > 1 else dim, st if t.shape[0] > 1 else heads * dim)
+    return shape[0], _strides2(sh if heads > 1 else dim, st if shape[0] > 1 else heads * dim)
 
 
-class _Seqs:
-    """Checked page table, lengths and prefix sums of one call."""
-    __slots__ = ("batch", "width", "stride", "table", "lens", "cu")
-
-    def __init__(self, page_table, seq_lens, cu_seqlens, device):
-        for name, t, dims in (("page_table", page_table, 2), ("seq_lens", seq_lens, 1), ("cu_seqlens", cu_seqlens, 1)):
-            if t is None and name == "cu_seqlens":
-                continue
+def _seqs(page_table, seq_lens, cu_seqlens, device):
+    """Checks the page table, lengths and prefix sums of a call; (table, its row stride, pages per sequence, lens, cu,
+    batch) as the C entry points take them."""
+    for name, t in (("page_table", page_table), ("seq_lens", seq_lens), ("cu_seqlens", cu_seqlens)):
+        if t is None and name == "cu_seqlens":
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype is not torch.int32 or t.device != device:
             _check_tensor(name, t, torch.int32)
-            if t.device != device:
-                raise ValueError(f"{name} is on {t.device}, the cache on {device}")
-            if t.dim() != dims:
-                raise ValueError(f"{name} must have {dims} dimension(s), got shape {tuple(t.shape)}")
-        self.batch, self.width = page_table.shape
-        if self.width == 0:
-            raise ValueError("page_table has no columns")
-        if self.width > 1 and page_table.stride(1) != 1:
-            raise ValueError("page_table: the pages of a sequence must be contiguous (stride 1)")
-        if seq_lens.shape[0] != self.batch or (self.batch > 1 and seq_lens.stride(0) != 1):
-            raise ValueError(f"seq_lens must be a contiguous vector of batch = {self.batch} entries")
-        if cu_seqlens is not None and (cu_seqlens.shape[0] != self.batch + 1 or cu_seqlens.stride(0) != 1):
-            raise ValueError(f"cu_seqlens must be a contiguous vector of batch + 1 = {self.batch + 1} entries")
-        self.stride = page_table.stride(0) if self.batch > 1 else self.width
-        self.table = page_table.data_ptr()
-        self.lens = seq_lens.data_ptr()
-        self.cu = None if cu_seqlens is None else cu_seqlens.data_ptr()
+            raise ValueError(f"{name} is on {t.device}, the cache on {device}")
+        dims = 2 if name == "page_table" else 1
+        if t.dim() != dims:
+            raise ValueError(f"{name} must have {dims} dimension(s), got shape {tuple(t.shape)}")
+    batch, width = page_table.shape
+    if width == 0:
+        raise ValueError("page_table has no columns")
+    stride, inner = page_table.stride()
+    if width > 1 and inner != 1:
+        raise ValueError("page_table: the pages of a sequence must be contiguous (stride 1)")
+    if seq_lens.shape[0] != batch or (batch > 1 and seq_lens.stride(0) != 1):
+        raise ValueError(f"seq_lens must be a contiguous vector of batch = {batch} entries")
+    if cu_seqlens is not None and (cu_seqlens.shape[0] != batch + 1 or cu_seqlens.stride(0) != 1):
+        raise ValueError(f"cu_seqlens must be a contiguous vector of batch + 1 = {batch + 1} entries")
+    return (page_table.data_ptr(), stride if batch > 1 else width, width, seq_lens.data_ptr(),
+            None if cu_seqlens is None else cu_seqlens.data_ptr(), batch)
 
 
 class PagedKVCache:
@@ -140,6 +156,8 @@ class PagedKVCache:
                                      strides(k), strides(v), _DTYPES[dtype],
                                      N.SAGE_CACHE_INT8 if self.storage == "int8" else N.SAGE_CACHE_16BIT)
         self._ref = ctypes.byref(self._c)
+        self._lib = N.load()
+        self._workspace = functools.lru_cache(maxsize=256)(functools.partial(self._lib.sage_paged_workspace_bytes, self._ref))
 
     @classmethod
     def empty(cls, num_pages, page_size, heads_kv, head_dim, dtype, device, *, storage="16bit", tensor_layout="HND",
@@ -166,11 +184,12 @@ class PagedKVCache:
         tv, vs = _packed2("v", v, self.heads_kv, self.head_dim, self.dtype, self.device)
         if tv != tokens:
             raise ValueError(f"k has {tokens} tokens, v {tv}")
-        s = _Seqs(page_table, seq_lens, cu_seqlens, self.device)
-        with torch.cuda.device(self.device):
-            rc = N.load().sage_paged_append(self._ref, k.data_ptr(), v.data_ptr(), ks, vs, s.table, s.stride, s.width,
-                                            s.lens, s.cu, s.batch, tokens, _stream_ptr(self.device))
-        N.check("sage_paged_append", rc)
+        s = _seqs(page_table, seq_lens, cu_seqlens, self.device)
+        with _on(self.device):
+            rc = self._lib.sage_paged_append(self._ref, k.data_ptr(), v.data_ptr(), ks, vs, *s, tokens,
+                                             _raw_stream(self.device.index))
+        if rc:
+            N.check("sage_paged_append", rc)
 
     def gather(self, page_table, seq_lens, cu_seqlens=None, *, total=None, out=None):
         """Read the newest tokens of each sequence back: (k, v), each [tokens, heads_kv, head_dim].
@@ -179,24 +198,26 @@ class PagedKVCache:
         ``total`` is its last entry, which the host has to know to allocate the result (default without
         cu_seqlens: one per sequence). ``out``: a pair of tensors to write into instead. Rows behind the
         last sequence are left as they are."""
-        s = _Seqs(page_table, seq_lens, cu_seqlens, self.device)
+        s = _seqs(page_table, seq_lens, cu_seqlens, self.device)
         if out is None:
             if total is None:
                 if cu_seqlens is not None:
                     raise ValueError("gather needs total (the number of tokens) or out")
-                total = s.batch
+                total = s[-1]
             shape = (int(total), self.heads_kv, self.head_dim)
-            k, v = (torch.empty(shape, dtype=self.dtype, device=self.device) for _ in range(2))
+            k = torch.empty(shape, dtype=self.dtype, device=self.device)
+            v = torch.empty(shape, dtype=self.dtype, device=self.device)
         else:
             k, v = out
         tokens, ks = _packed2("out[0]", k, self.heads_kv, self.head_dim, self.dtype, self.device)
         tv, vs = _packed2("out[1]", v, self.heads_kv, self.head_dim, self.dtype, self.device)
         if tv != tokens or (total is not None and tokens != int(total)):
             raise ValueError(f"out holds {tokens} and {tv} tokens, expected {tokens if total is None else int(total)}")
-        with torch.cuda.device(self.device):
-            rc = N.load().sage_paged_gather(self._ref, k.data_ptr(), v.data_ptr(), ks, vs, s.table, s.stride, s.width,
-                                            s.lens, s.cu, s.batch, tokens, _stream_ptr(self.device))
-        N.check("sage_paged_gather", rc)
+        with _on(self.device):
+            rc = self._lib.sage_paged_gather(self._ref, k.data_ptr(), v.data_ptr(), ks, vs, *s, tokens,
+                                             _raw_stream(self.device.index))
+        if rc:
+            N.check("sage_paged_gather", rc)
         return k, v
 
 
@@ -216,29 +237,30 @@ def run_paged_attn(q, cache: PagedKVCache, page_table, seq_lens, cu_seqlens_q=No
     """
     if not isinstance(cache, PagedKVCache):
         raise TypeError("cache must be a PagedKVCache")
-    _check_tensor("q", q, cache.dtype)
-    if q.dim() != 3:
+    if not isinstance(q, torch.Tensor) or q.dim() != 3:
+        _check_tensor("q", q, cache.dtype)
         raise ValueError(f"q must be a packed [tokens, heads, head_dim] tensor, got shape {tuple(q.shape)}")
+    device, dim = cache.device, cache.head_dim
     heads = q.shape[1]
-    total, qs = _packed2("q", q, heads, cache.head_dim, cache.dtype, cache.device)
-    s = _Seqs(page_table, seq_lens, cu_seqlens_q, cache.device)
+    total, qs = _packed2("q", q, heads, dim, cache.dtype, device)
+    s = _seqs(page_table, seq_lens, cu_seqlens_q, device)
     if out is None:
-        out = torch.empty((total, heads, cache.head_dim), dtype=q.dtype, device=cache.device)
-    to, os_ = _packed2("out", out, heads, cache.head_dim, cache.dtype, cache.device)
+        out = torch.empty((total, heads, dim), dtype=cache.dtype, device=device)
+    to, os_ = _packed2("out", out, heads, dim, cache.dtype, device)
     if to != total:
         raise ValueError(f"out shape {tuple(out.shape)} differs from q {tuple(q.shape)}")
     if max_seqlen_q is None:
         max_seqlen_q = max(total, 1) if cu_seqlens_q is not None else 1
-    if window is not None and window <= 0:
+    if window is None:
+        window = 0
+    elif window <= 0:
         raise ValueError(f"window must be positive, got {window}")
-    lib = N.load()
-    ref = cache._ref
-    with torch.cuda.device(cache.device):
-        n = lib.sage_paged_workspace_bytes(ref, heads, s.batch, total, max_seqlen_q, s.width)
-        ws = torch.empty(max(n, 1), dtype=torch.uint8, device=cache.device)
-        rc = lib.sage_paged_attn_fwd(ref, q.data_ptr(), qs, out.data_ptr(), os_, heads, s.table, s.stride, s.width, s.lens,
-                                     s.cu, s.batch, total, max_seqlen_q, int(bool(causal)), window or 0, sinks,
-                                     0.0 if sm_scale is None else float(sm_scale), ws.data_ptr(), n,
-                                     _stream_ptr(cache.device))
-    N.check("sage_paged_attn_fwd", rc)
+    with _on(device):
+        n = cache._workspace(heads, s[-1], total, max_seqlen_q, s[2])
+        ws = torch.empty(n or 1, dtype=torch.uint8, device=device)
+        rc = cache._lib.sage_paged_attn_fwd(cache._ref, q.data_ptr(), qs, out.data_ptr(), os_, heads, *s, total, max_seqlen_q,
+                                            1 if causal else 0, window, sinks, 0.0 if sm_scale is None else sm_scale,
+                                            ws.data_ptr(), n, _raw_stream(device.index))
+    if rc:
+        N.check("sage_paged_attn_fwd", rc)
     return out
