@@ -24,7 +24,7 @@ int check_cache(const sage_paged_cache* c) {
     if (c->k_strides[i] <= 0 || c->k_strides[i] % unit || c->v_strides[i] <= 0 || c->v_strides[i] % unit)
       return fail(SAGE_ERR_INVALID_ARG, "cache stride[%d] (k %lld, v %lld) must be a positive multiple of %lld elements",
                   i, (long long)c->k_strides[i], (long long)c->v_strides[i], (long long)unit);
-    if (c->k_strides[i] > (1LL << 38) || c->v_strides[i] > (1LL << 38))
+    if (c->k_strides[i] > (1LL << 34) || c->v_strides[i] > (1LL << 34))
       return fail(SAGE_ERR_INVALID_ARG, "cache stride[%d] is too large", i);
   }
   if (!c->k || !c->v || (i8 && (!c->k_scale || !c->v_scale))) return fail(SAGE_ERR_INVALID_ARG, "NULL cache pointer");
@@ -132,14 +132,15 @@ size_t decode_ws_bytes(int64_t D) {
 
 // Tensor maps of the cache's K or V ([pages][heads][page][D], boxes of at most `rows` tokens) and of
 // its scales ([pages][heads][page]).
-int cache_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows) {
+int cache_map(CUtensorMap* map, const sage_paged_cache* c, bool v, int rows, bool swizzle = true) {
   const int64_t* s = v ? c->v_strides : c->k_strides;
   const void* base = v ? c->v : c->k;
   const uint32_t box = (uint32_t)std::min<int64_t>(rows, c->page_size);
   if (c->storage == SAGE_CACHE_INT8)
     return encode_4d(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, base, c->head_dim, c->page_size, c->heads_kv, c->num_pages,
                      s[2], s[1], s[0], (uint32_t)c->head_dim, box,
-                     c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+                     !swizzle ? CU_TENSOR_MAP_SWIZZLE_NONE
+                     : c->head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
   return encode_4d(map, c->dtype == SAGE_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
                    2, base, c->head_dim, c->page_size, c->heads_kv, c->num_pages, s[2], s[1], s[0], 64, box,
                    CU_TENSOR_MAP_SWIZZLE_128B);
@@ -342,8 +343,9 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   const bool chunk = chunk_route(max_seqlen_q, G);
   const int tile = chunk ? 128 : sage::kDecKeys;  // keys of a tile
   PagedMaps m;
-  if (int rc = cache_map(&m.k, c, false, tile)) return rc;
-  if (int rc = cache_map(&m.v, c, true, tile)) return rc;
+  // the chunk kernel widens INT8 codes itself, from rows as they are
+  if (int rc = cache_map(&m.k, c, false, tile, !chunk)) return rc;
+  if (int rc = cache_map(&m.v, c, true, tile, !chunk)) return rc;
   if (chunk) {
     sage::ChunkParams cp{};
     const int64_t items = chunk_items(batch, total_q, G);

@@ -24,10 +24,16 @@
 // follows the largest v_scale of the segment (E is raised, and O rescaled, once a tile exceeds it by
 // 2^4; P < 2^8 * 2^5 stays inside fp16). bf16 queries are brought to fp16 by a power of two per row.
 //
+// Code size counts: the softmax's and the converters' loops run side by side on the same instruction
+// cache, and unrolled whole (22 KB of converter) the INT8 kernel took 475 us where this one takes 343
+// (two chunks of 1024 over 7168, 32/8 heads, head_dim 128). For the same reason every exponential is
+// MUFU.ex2: the polynomial share that sage_attn.cuh computes on the FMA pipe costs more here (12 of 32
+// columns: 16 bit 243 -> 231 us, INT8 540 -> 475 us without).
+//
 // Warps: 0-7 softmax (two warpgroups), 8 TMA producer of K and V, 9 MMA issuer, 10 loads the next
 // segment's queries as soon as the last Q K^T of this one has run, 11 puts zeros over rows of V that no
 // query sees (an unused row may hold a NaN, which its weight of 0 would not silence). INT8: 8 loads
-// queries and scales, 10 converts K, 11 converts V.
+// the queries too, 10 converts K, 11 converts V and brings the scales.
 #pragma once
 
 #include "sage_attn.cuh"
@@ -76,15 +82,17 @@ struct ChunkCfg {
   static constexpr int OUT_BYTES = 32 * OUT_CH * 2;          // per softmax warp: 32 rows of them
   static constexpr int OFF_OUT = OFF_V + NS * TILE;
   static constexpr int OFF_BAR = OFF_OUT + 8 * OUT_BYTES;
-  static constexpr int NUM_BARS = 3 + 6 * NS + 12;
+  static constexpr int NUM_BARS = 3 + 7 * NS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
-  static constexpr int OFF_WALK = (OFF_MISC + 8 + 15) / 16 * 16;  // where each softmax warp is in the piece
-  static constexpr int WALK_BYTES = 96;
-  static constexpr int OFF_SCALE = (OFF_WALK + 8 * WALK_BYTES + 15) / 16 * 16;  // INT8: per stage k_scale, v_scale 2^-E
+  static constexpr int OFF_WALK = (OFF_MISC + 8 + 15) / 16 * 16;  // where each warp is in the piece
+  static constexpr int WALK_BYTES = 80;
+  static constexpr int OFF_SCALE = (OFF_WALK + 12 * WALK_BYTES + 15) / 16 * 16;  // INT8: per stage k_scale, v_scale 2^-E
   static constexpr int OFF_EXP = OFF_SCALE + (I8 ? NS * 1024 : 0);               // and E
   static constexpr int SMEM_BYTES = 1024 + OFF_EXP + (I8 ? 16 : 0);
   static_assert(SMEM_BYTES <= 227 * 1024 && SMEM_BYTES > 114 * 1024, "one CTA per SM");
-  static constexpr int REGS_SOFTMAX = 216, REGS_OTHER = 72;  // as in AttnCfg
+  // 256 softmax and 128 other threads share 384 x 168 registers; a converter keeps 32 registers of loads in flight
+  static constexpr int REGS_SOFTMAX = I8 ? 208 : 216, REGS_OTHER = I8 ? 88 : 72;
+  static_assert(256 * REGS_SOFTMAX + 128 * REGS_OTHER <= 384 * 168, "register split");
   static constexpr uint32_t QK_LAYOUT = kLayoutSW128, QK_SBO = 1024;
   static constexpr int QK_STEPS = D / 16;
   static __device__ __forceinline__ uint32_t qk_step_offset(int kk, int rows) {
@@ -98,7 +106,6 @@ struct ChunkCfg {
   static constexpr uint32_t IDESC_QK = make_idesc(kFmtD_F32, FMT, FMT, 0, 0, BM, BN);
   static constexpr uint32_t IDESC_PV = make_idesc(kFmtD_F32, FMT, FMT, 0, 1, BM, D);
   static constexpr float LAZY = 8.0f;
-  static constexpr int EMU = 12;
 };
 
 // ------------------------------------------------------------------ schedule
@@ -239,6 +246,7 @@ struct ChunkWalk {
   bool go;
   ChunkItem it;
   int n;
+  ChunkWalk() = default;
   __device__ __forceinline__ ChunkWalk(const ChunkParams& p, int cta) {
     const int4 a = reinterpret_cast<const int4*>(p.pieces + cta)[0], z = reinterpret_cast<const int4*>(p.pieces + cta)[1];
     items = p.items;
@@ -293,6 +301,18 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
 // The lowest n bits (n may be anything).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
+__device__ __forceinline__ void st_shared_v4(uint32_t dst, const uint4& v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(dst), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t src) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src) : "memory");
+  return v;
+}
+__device__ __forceinline__ void ld_shared_f4(uint32_t src, float2 (&v)[2]) {
+  asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];"
+               : "=l"(reinterpret_cast<uint64_t&>(v[0])), "=l"(reinterpret_cast<uint64_t&>(v[1])) : "r"(src));
+}
 // One 16-byte piece of INT8 codes as 16 fp16 values: 32 bytes, as two 16-byte units.
 __device__ __forceinline__ void codes_to_half16(const uint4& w, uint4& a, uint4& z) {
   const uint32_t x = w.x ^ 0x80808080u, y = w.y ^ 0x80808080u, u = w.z ^ 0x80808080u, v = w.w ^ 0x80808080u;
@@ -327,7 +347,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* bar_sload = bar_odone + 2;
   uint64_t* bar_pvdone = bar_sload + 2;
   uint64_t* bar_sc = bar_pvdone + 2;    // [stage] INT8: the tile's scales are in place
-  uint64_t* bar_qraw = bar_sc + C::NS;  // bf16 queries landed, to be converted by the softmax threads
+  uint64_t* bar_kraw = bar_sc + C::NS;  // [stage] INT8: K's codes landed (V's: bar_vraw)
+  uint64_t* bar_qraw = bar_kraw + C::NS;  // bf16 queries landed, to be converted by the softmax threads
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   const uint32_t warp = warp_id(), lane = lane_id();
@@ -340,6 +361,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     for (int s = 0; s < C::NS; ++s) {
       mbar_init(bar_vraw + s, 1);
       mbar_init(bar_sc + s, 1);
+      mbar_init(bar_kraw + s, 1);
       mbar_init(bar_kfull + s, 1);
       mbar_init(bar_vfull + s, 1);
       mbar_init(bar_kempty + s, 1);
@@ -360,7 +382,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     tmem_alloc(tmem_slot, 512);
     tmem_relinquish();
   }
-  if (!I8 && warp == 8 && lane == 0) {
+  if (warp == 8 && lane == 0) {
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
@@ -370,9 +392,28 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   const uint32_t tmem_base = *tmem_slot;
   asm volatile("griddepcontrol.wait;" ::: "memory");  // the schedule is written
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // The walk through the piece. In the softmax warps, and in those that convert INT8, it lives in shared
+  // memory: its registers would spill beside a row of 128 scores, or beside the loads in flight.
+  static_assert(sizeof(ChunkWalk) <= C::WALK_BYTES, "walk");
+  ChunkWalk* const shared_walk = reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * C::WALK_BYTES);
+  auto shared_next = [&] {
+    __syncwarp();
+    if (lane == 0) shared_walk->next();
+    __syncwarp();
+  };
+  if (I8 || warp < 8) {
+    if (lane == 0) *shared_walk = ChunkWalk(cp, cta);
+    __syncwarp();
+  }
   if (warp >= 8) {
     regs_dec<C::REGS_OTHER>();
-    ChunkWalk w(cp, cta);
+    ChunkWalk own;
+    if constexpr (!I8) own = ChunkWalk(cp, cta);
+    ChunkWalk& w = I8 ? *shared_walk : own;
+    auto step = [&] {
+      if constexpr (I8) shared_next();
+      else own.next();
+    };
     // first key behind those that some query of the segment sees, and first of its window
   auto seen = [&](int* hi, int* lo) {
     const int first = w.it.len - w.it.n + w.first_tok(cp);
@@ -405,135 +446,105 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       const int pg = (w.key0(tj) >> p.page_shift) + (int)lane % ppt;
       return pg < p.s.width ? p.s.table[(int64_t)w.it.b * p.s.table_stride + pg] : -1;
     };
-    if (I8 && warp == 8) {
-      // ------------------------------------------------------------ queries and scales
-      const int sh = min(p.page_shift, 7);
+    if (I8 && warp >= 10) {
+      // ------------------------------------------------------------ codes to fp16 tiles: K (warp 10), V (warp 11)
+      // The codes land in the upper half of their slot and are widened in place: at head_dim 128 row r's
+      // codes lie where the upper half of its fp16 values goes; at 64 rows are taken in order, and the
+      // values of rows up to r cover codes of rows up to r only. A group of rows is read whole, then
+      // written. Codes that nobody sees are finite whatever they are, so their weight of 0 suffices.
+      // Warp 11 also brings the scales: k_scale, and v_scale in units of 2^E.
+      const bool isv = warp == 11;
+      constexpr int LPR = D / 16, RPI = 32 / LPR;  // lanes per row of codes, rows per pass
+      constexpr int NG = 128 / (8 * RPI);          // groups of eight passes
+      // Lane: 16 codes c of row `sub` of every RPI rows. At head_dim 128 the upper half's lanes take the
+      // neighbouring row, so that the eight lanes of a store phase hit eight different 16-byte banks.
+      const int c = lane % LPR, sub = (lane / LPR) ^ (D == 128 ? c >> 2 : 0), sh = min(p.page_shift, 7);
+      uint64_t* bar_full = isv ? bar_vfull : bar_kfull;
+      uint64_t* bar_raw = isv ? bar_vraw : bar_kraw;
+      const uint32_t slots = smem_u32(smem + (isv ? C::OFF_V : C::OFF_K));
+      const uint32_t src = slots + C::TILE / 2 + sub * D + c * 16;
+      // a row's two 16-byte units (2 c, 2 c + 1 of 8 per 128-byte atom), rows of even and odd passes
+      const int unit = 2 * (c & 3);
+      const uint32_t dst = slots + (c >> 2) * (128 * 128) + sub * 128;
+      const uint32_t off0 = (unit ^ (sub & 7)) << 4, off1 = (unit ^ ((RPI + sub) & 7)) << 4;
       int it = 0;
       bool ok = true;
-      for (int seg = 0; w.more() && ok; w.next(), ++seg) {
-        if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-        if (lane == 0) load_queries();
-        __syncwarp();
-        const int kvh = w.head / p.parts;
+      for (; w.more() && ok; step()) {
+        const int n = w.n, kvh = w.head / p.parts;
         int hi, lo, ids = 0, e = -200;
         seen(&hi, &lo);
-        for (int j = 0; j < w.n; ++j, ++it) {
-          const int s = it % C::NS, key0 = w.key0(j), key = key0 + 4 * lane;
-          if (j % batch_tiles == 0) ids = page_of(j);
-          const int id = __shfl_sync(0xffffffffu, ids, (j % batch_tiles) * ppt + ((4 * lane) >> sh));
+        for (int j = 0; j < n; ++j, ++it) {
+          const int s = it % C::NS;
           float k4[4] = {0.f, 0.f, 0.f, 0.f}, v4[4] = {0.f, 0.f, 0.f, 0.f};
-          if (id >= 0 && id < cp.c.pages) {
-            const int64_t at = (((int64_t)id * cp.c.heads + kvh) << p.page_shift) + (key & (page - 1));
-            const float4 a = *reinterpret_cast<const float4*>(cp.c.k_scale + at), z = *reinterpret_cast<const float4*>(cp.c.v_scale + at);
-            k4[0] = a.x; k4[1] = a.y; k4[2] = a.z; k4[3] = a.w;
-            v4[0] = z.x; v4[1] = z.y; v4[2] = z.z; v4[3] = z.w;
-          }
-          float m = 0.0f;
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int kx = key + x;
-            if (!(kx < hi && (kx >= lo || kx < p.sinks))) k4[x] = v4[x] = 0.0f;
-            m = fmaxf(m, v4[x]);
-          }
-#pragma unroll
-          for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-          // exponent of the largest scale (a negative one never arises from the cache's own writes)
-          const int et = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 120);
-          if (e == -200 || et > e + 4) e = et;
-          const float down = pow2(-e);
-          if (it >= C::NS) ok = mbar_wait(bar_vempty + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
-          float4* dst = reinterpret_cast<float4*>(smem + C::OFF_SCALE + s * 1024);
-          dst[lane] = make_float4(k4[0], k4[1], k4[2], k4[3]);
-          dst[32 + lane] = make_float4(v4[0] * down, v4[1] * down, v4[2] * down, v4[3] * down);
-          if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = e;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(bar_sc + s);
-        }
-      }
-    } else if (I8 && warp >= 10) {
-      // ------------------------------------------------------------ codes to fp16 tiles: K (warp 10), V (warp 11)
-      const bool isv = warp == 11;
-      constexpr int LPR = D / 16, RPI = 32 / LPR;  // lanes per row of codes, rows per iteration
-      constexpr int NG = 128 / (8 * RPI);          // groups of eight iterations per tile
-      const int c = lane % LPR, sub = lane / LPR, sh = min(p.page_shift, 7);
-      const char* base = static_cast<const char*>(isv ? cp.c.v : cp.c.k);
-      const int64_t sp = isv ? cp.c.v_sp : cp.c.k_sp, sr = isv ? cp.c.v_st : cp.c.k_st;
-      uint64_t* bar_full = isv ? bar_vfull : bar_kfull;
-      uint64_t* bar_empty = isv ? bar_vempty : bar_kempty;
-      uint8_t* tiles = smem + (isv ? C::OFF_V : C::OFF_K);
-      // state of the loads, which run one group (and so up to one tile) ahead of the conversion
-      int j = 0, ids = 0, key0 = 0, hi = 0, lo = 0;
-      const char* head_base = base;
-      auto enter = [&](bool segment) {  // the tile j of the present segment
-        if (segment) {
-          seen(&hi, &lo);
-          head_base = base + (int64_t)(w.head / p.parts) * (isv ? cp.c.v_sh : cp.c.k_sh) + c * 16;
-        }
-        if (j % batch_tiles == 0) ids = page_of(j);
-        key0 = w.key0(j);
-      };
-      auto load = [&](int row) {
-        const int id = __shfl_sync(0xffffffffu, ids, (j % batch_tiles) * ppt + (row >> sh));
-        const int key = key0 + row;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (w.more() && id >= 0 && id < cp.c.pages && key < hi && (key >= lo || key < p.sinks))
-          x = ldg_nc_v4(head_base + (int64_t)id * sp + (int64_t)(key & (page - 1)) * sr);
-        return x;
-      };
-      uint4 reg[8];
-      bool more = w.more(), ok = true;
-      if (more) {
-        enter(true);
-#pragma unroll
-        for (int u = 0; u < 8; ++u) reg[u] = load(u * RPI + sub);
-      }
-      for (int it = 0; more && ok; ++it) {
-        const int s = it % C::NS;
-        if (it >= C::NS) ok = mbar_wait(bar_empty + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
-        ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
-#pragma unroll 1
-        for (int g = 0; g < NG; ++g) {
-          if (g == NG - 1) {  // the next loads are the next tile's
-            if (++j == w.n) {
-              w.next();
-              j = 0;
-              more = w.more();
-              if (more) enter(true);
-            } else {
-              enter(false);
+          const int key = w.key0(j) + 4 * lane;
+          if (isv) {
+            if (j % batch_tiles == 0) ids = page_of(j);
+            const int id = __shfl_sync(0xffffffffu, ids, (j % batch_tiles) * ppt + ((4 * lane) >> sh));
+            if (id >= 0 && id < cp.c.pages) {
+              const int64_t at = (((int64_t)id * cp.c.heads + kvh) << p.page_shift) + (key & (page - 1));
+              const float4 a = *reinterpret_cast<const float4*>(cp.c.k_scale + at), z = *reinterpret_cast<const float4*>(cp.c.v_scale + at);
+              k4[0] = a.x; k4[1] = a.y; k4[2] = a.z; k4[3] = a.w;
+              v4[0] = z.x; v4[1] = z.y; v4[2] = z.z; v4[3] = z.w;
             }
           }
-          const int next = g == NG - 1 ? 0 : g + 1;
+          ok = mbar_wait(bar_raw + s, (it / C::NS) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (isv) {  // V's slot is free, so are the scales'
+            float m = 0.0f;
 #pragma unroll
-          for (int u = 0; u < 8; ++u) {
-            const int row = (g * 8 + u) * RPI + sub;
-            uint4 a, z;
-            codes_to_half16(reg[u], a, z);
-            reg[u] = load((next * 8 + u) * RPI + sub);
-            // units 2 c and 2 c + 1 of the row's 16-byte units, 8 per 128-byte atom; the upper atom's
-            // lanes store theirs in the other order, against bank conflicts
-            const bool odd = D == 128 && c >= 4;
-            uint8_t* dst = tiles + s * C::TILE + (c >> 2) * (128 * 128) + row * 128;
-            const int u0 = 2 * (c & 3) + (odd ? 1 : 0), u1 = u0 ^ 1;
-            *reinterpret_cast<uint4*>(dst + ((u0 ^ (row & 7)) << 4)) = odd ? z : a;
-            *reinterpret_cast<uint4*>(dst + ((u1 ^ (row & 7)) << 4)) = odd ? a : z;
+            for (int x = 0; x < 4; ++x) {
+              const int kx = key + x;
+              if (!(kx < hi && (kx >= lo || kx < p.sinks))) k4[x] = v4[x] = 0.0f;
+              m = fmaxf(m, v4[x]);
+            }
+#pragma unroll
+            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const int et = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 120);
+            if (e == -200 || et > e + 4) e = et;
+            const float down = pow2(-e);
+            float4* sc = reinterpret_cast<float4*>(smem + C::OFF_SCALE + s * 1024);
+            sc[lane] = make_float4(k4[0], k4[1], k4[2], k4[3]);
+            sc[32 + lane] = make_float4(v4[0] * down, v4[1] * down, v4[2] * down, v4[3] * down);
+            if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = e;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_sc + s);
           }
+#pragma unroll 1
+          for (int g = 0; g < NG; ++g) {
+            uint4 x[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) x[u] = ld_shared_v4(src + s * C::TILE + (g * 8 + u) * (RPI * D));
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+              uint4 a, z;
+              codes_to_half16(x[u], a, z);
+              const uint32_t o = dst + s * C::TILE + (g * 8 + u) * (RPI * 128) + ((u & 1) ? off1 : off0);
+              st_shared_v4(o, a);
+              st_shared_v4(o ^ 16, z);
+            }
+            __syncwarp();
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(bar_full + s);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(bar_full + s);
       }
     } else if (warp == 8) {
       // ------------------------------------------------------------ TMA producer
-      const int boxes = ppt * C::ATOMS;  // of K, and of V
+      // boxes of K, and of V: one per page and 128-byte atom (INT8: per page, into the slot's upper half)
+      const int boxes = I8 ? ppt : ppt * C::ATOMS;
       int it = 0;
       bool ok = true;
-      for (; w.more() && ok; w.next()) {
+      for (int seg = 0; w.more() && ok; step(), ++seg) {
+        if constexpr (I8) {  // the queries too: warp 10 converts
+          if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          if (lane == 0) load_queries();
+          __syncwarp();
+        }
         const int kvh = w.head / p.parts;
         int next = page_of(0);
         for (int j0 = 0; j0 < w.n && ok; j0 += batch_tiles) {
@@ -545,8 +556,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const int key0 = w.key0(j), y = key0 & (page - 1);
             const int sub = lane % ppt, atom = lane / ppt;
             const int id = __shfl_sync(0xffffffffu, ids, (j - j0) * ppt + sub);
-            const int dst = s * C::TILE + atom * (128 * 128) + sub * rows * 128;
-            uint64_t* vbar = (ragged(key0) ? bar_vraw : bar_vfull) + s;
+            const int dst = s * C::TILE + (I8 ? C::TILE / 2 + sub * rows * D : atom * (128 * 128) + sub * rows * 128);
+            uint64_t* vbar = (I8 || ragged(key0) ? bar_vraw : bar_vfull) + s;
 #pragma unroll
             for (int isv = 0; isv < 2; ++isv) {
               if (ok && it >= C::NS)
@@ -554,8 +565,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                                p.wait_limit_ns);
               ok = __all_sync(0xffffffffu, ok);
               if (!ok) break;
-              uint64_t* bar = isv ? vbar : bar_kfull + s;
-              if (lane == 0) mbar_arrive_expect_tx(bar, C::TILE);
+              uint64_t* bar = isv ? vbar : (I8 ? bar_kraw : bar_kfull) + s;
+              if (lane == 0) mbar_arrive_expect_tx(bar, I8 ? C::TILE / 2 : C::TILE);
               __syncwarp();
               if (lane < boxes)
                 tma_load_4d(smem + (isv ? C::OFF_V : C::OFF_K) + dst, isv ? &tmV : &tmK, bar, atom * 64, y, kvh, id);
@@ -567,7 +578,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if (!ok) {  // gave up: wait (bounded) for the copies of K in flight (those of V were issued with them)
         for (int j = max(0, it - C::NS); j < it; ++j) {
           volatile int none = 0;
-          (void)mbar_wait(bar_kfull + j % C::NS, (j / C::NS) & 1, &none, kDevTimeoutProducer, p.wait_limit_ns);
+          (void)mbar_wait((I8 ? bar_kraw : bar_kfull) + j % C::NS, (j / C::NS) & 1, &none, kDevTimeoutProducer, p.wait_limit_ns);
         }
       }
     } else if (warp == 9) {
@@ -668,7 +679,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       int it = 0;
       uint32_t raw_phase = 0;  // bit s: phase of bar_vraw[s]
       bool ok = true;
-      for (; w.more() && ok; w.next()) {
+      for (; w.more() && ok; step()) {
         int hi, lo;
         seen(&hi, &lo);
         for (int j = 0; j < w.n && ok; ++j, ++it) {
@@ -711,18 +722,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     int ct = 0, segs = 0;  // tiles and segments of this query tile so far
     int it0 = 0, qseg = 0;  // tiles and segments of the CTA so far
     bool ok = true;
-    // The walk through the piece lives in shared memory, one per warp: its fifteen registers beside a
-    // row of 128 scores would spill.
-    static_assert(sizeof(ChunkWalk) <= C::WALK_BYTES, "walk");
-    ChunkWalk& w = *reinterpret_cast<ChunkWalk*>(smem + C::OFF_WALK + warp * C::WALK_BYTES);
-    if (lane == 0) w = ChunkWalk(cp, cta);
-    __syncwarp();
-    auto step = [&] {
-      __syncwarp();
-      if (lane == 0) w.next();
-      __syncwarp();
-    };
-    for (; ok && w.more(); step()) {
+    ChunkWalk& w = *shared_walk;
+    for (; ok && w.more(); shared_next()) {
       const int first_tok = w.first_tok(cp) + t * p.TT;           // of this query tile
       const int toks = min(p.TT, w.it.n - first_tok);
       const int n = w.n, it_seg = it0;
@@ -733,26 +734,25 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         if (!__all_sync(0xffffffffu, mbar_wait(bar_qraw, qseg++ & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
         if (toks > 0) {
           uint8_t* q = smem + C::OFF_Q + t * C::TILE + row_in_tile * 128;
+          auto piece = [&](int x) { return reinterpret_cast<uint4*>(q + (x >> 3) * (128 * 128) + (((x & 7) ^ (row_in_tile & 7)) << 4)); };
           uint32_t m = 0;
-          uint4 raw[D / 8];
-#pragma unroll
+#pragma unroll 2
           for (int x = 0; x < D / 8; ++x) {
-            raw[x] = *reinterpret_cast<uint4*>(q + (x >> 3) * (128 * 128) + (((x & 7) ^ (row_in_tile & 7)) << 4));
             float f[8];
-            Half8<T>::to_float(raw[x], f);
+            Half8<T>::to_float(*piece(x), f);
 #pragma unroll
             for (int y = 0; y < 8; ++y) m = max(m, abs_bits(f[y]));
           }
           const int e = min(max((int)(m >> 23) - 127, -126), 126);
           const float down = pow2(-e);
           scale *= pow2(e);
-#pragma unroll
+#pragma unroll 2
           for (int x = 0; x < D / 8; ++x) {
             float f[8];
-            Half8<T>::to_float(raw[x], f);
+            Half8<T>::to_float(*piece(x), f);
 #pragma unroll
             for (int y = 0; y < 8; ++y) f[y] *= down;
-            *reinterpret_cast<uint4*>(q + (x >> 3) * (128 * 128) + (((x & 7) ^ (row_in_tile & 7)) << 4)) = Half8<__half>::from_float(f);
+            *piece(x) = Half8<__half>::from_float(f);
           }
         }
         fence_proxy_async_smem();
@@ -784,26 +784,31 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           for (int c = 0; c < 128; ++c) b[c] = __uint_as_float(sr[c]);
         }
         float shrink = 1.0f;  // INT8: O's factor where the unit is raised
-        const float4* scales = nullptr;
+        uint32_t scales = 0;
         if constexpr (I8) {
           const int s = (it_seg + j) % C::NS;
           if (!__all_sync(0xffffffffu, mbar_wait(bar_sc + s, ((it_seg + j) / C::NS) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
-          scales = reinterpret_cast<const float4*>(smem + C::OFF_SCALE + s * 1024);
-          const int e = reinterpret_cast<const int*>(smem + C::OFF_EXP)[s];
+          scales = smem_u32(smem + C::OFF_SCALE) + s * 1024;
+          const int e = *reinterpret_cast<const int*>(smem + C::OFF_EXP + 4 * s);
+          float2 ks4[4][2];
           if (j > 0 && e != e_run) shrink = pow2(max(e_run - e, -126));
           e_run = e;
 #pragma unroll
           for (int c = 0; c < 128; c += 4) {
-            const float4 ks = scales[c / 4];
-            const float2 x = fmul2(make_float2(b[c], b[c + 1]), make_float2(ks.x, ks.y));
-            const float2 y = fmul2(make_float2(b[c + 2], b[c + 3]), make_float2(ks.z, ks.w));
+            if (c % 16 == 0) {
+#pragma unroll
+              for (int x = 0; x < 4; ++x) ld_shared_f4(scales + 4 * c + 16 * x, ks4[x]);
+            }
+            const float2* ks = ks4[c / 4 % 4];
+            const float2 x = fmul2(make_float2(b[c], b[c + 1]), ks[0]);
+            const float2 y = fmul2(make_float2(b[c + 2], b[c + 3]), ks[1]);
             b[c] = x.x; b[c + 1] = x.y; b[c + 2] = y.x; b[c + 3] = y.y;
           }
         }
         const int up = hi - key0, down = lo - key0, sk = p.sinks - key0;
         const bool masked = key0 + 128 > all_hi || (key0 < all_lo && key0 + 128 > p.sinks);
-        uint32_t vis[4];  // bit c % 32 of word c / 32: this row sees key c of the tile
         if (masked) {
+          uint32_t vis[4];  // bit c % 32 of word c / 32: this row sees key c of the tile
 #pragma unroll
           for (int x = 0; x < 4; ++x)
             vis[x] = low_bits(up - 32 * x) & (~low_bits(down - 32 * x) | low_bits(sk - 32 * x));
@@ -833,33 +838,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) {
           uint32_t pk[32];
+          float2 vs[2][2];  // INT8: v_scale of four columns, and of the next four
+          if constexpr (I8) ld_shared_f4(scales + 512 + 256 * h2, vs[0]);
 #pragma unroll
           for (int pr = 0; pr < 32; ++pr) {
             const int c = h2 * 64 + 2 * pr;
+            if (I8 && pr % 2 == 0 && pr < 30) ld_shared_f4(scales + 528 + 4 * c, vs[(pr / 2 + 1) % 2]);
             const float2 a = ffma2(make_float2(b[c], b[c + 1]), scv, ccv);
-            float2 e;
-            if ((c % 32) >= 32 - C::EMU) {
-              e = exp2_poly2(a);
-            } else {
-              e.x = ex2_approx(a.x);
-              e.y = ex2_approx(a.y);
-            }
+            float2 e = make_float2(ex2_approx(a.x), ex2_approx(a.y));
             acc[pr & 3] = fadd2(acc[pr & 3], e);
-            if constexpr (I8) {
-              const float2 vs = reinterpret_cast<const float2*>(scales + 32)[c / 2];
-              e = fmul2(e, vs);
-            }
+            if constexpr (I8) e = fmul2(e, vs[pr / 2 % 2][pr % 2]);
             pk[pr] = pack2<M>(e.x, e.y);
-          }
-          // the polynomial's least result, 2^-125, is no zero in bf16
-          if (std::is_same<M, __nv_bfloat16>::value && masked) {
-#pragma unroll
-            for (int pr = 0; pr < 32; ++pr) {
-              const int c = h2 * 64 + 2 * pr;
-              if ((c % 32) < 32 - C::EMU) continue;
-              const uint32_t v = vis[c / 32] >> (c % 32);
-              pk[pr] &= ((v & 1u) ? 0xffffu : 0u) | ((v & 2u) ? 0xffff0000u : 0u);
-            }
           }
           if (h2 == 1) {
             tmem_st_wait();
@@ -871,7 +860,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           }
           tmem_st32(s_tmem + C::P_COL + 32 * h2, *reinterpret_cast<uint32_t(*)[32]>(&pk[0]));
           if (h2 == 0 && rescale) {
-#pragma unroll
+#pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
               uint32_t orow[32];
               tmem_ld32_sync(o_tmem + c0, orow);
@@ -910,7 +899,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         T* out = static_cast<T*>(p.o) + (int64_t)(w.it.base + first_tok) * p.o_st +
                  (int64_t)(kvh * p.G + part * p.Gp) * p.o_sh;
         const int piece = lane % PR;
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += C::OUT_CH) {
 #pragma unroll
           for (int h2 = 0; h2 < C::OUT_CH / 32; ++h2) {
@@ -938,7 +927,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       } else {
         // channels 4 x .. 4 x + 3 of row r at [x][r], so that a warp's store is contiguous
         float4* dst = reinterpret_cast<float4*>(p.part) + slot * kChunkRows * (D / 4) + row;
-#pragma unroll
+#pragma unroll 1
         for (int c0 = 0; c0 < D; c0 += 32) {
           uint32_t orow[32];
           tmem_ld32_sync(o_tmem + c0, orow);
