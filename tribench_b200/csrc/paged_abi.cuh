@@ -126,8 +126,8 @@ int paged_move(const sage_paged_cache* c, const void* k, const void* v, const in
 
 // ---------------------------------------------------------------- attention over the cache
 size_t decode_ws_bytes(int64_t D) {
-  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
-  return align256(rows * D * 4) + align256(rows * 4 * 4) + align256(sizeof(int4) * sage::kDecPieces);
+  const size_t rows = size_t(2) * sage::kDecMaxPieces * sage::kDecMaxRows;
+  return align256(rows * D * 4) + align256(rows * 4 * 4) + align256(sizeof(int4) * sage::kDecMaxPieces);
 }
 
 // Tensor maps of the cache's K or V ([pages][heads][page][D], boxes of at most `rows` tokens) and of
@@ -180,7 +180,7 @@ int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q 
 
 // Which kernel: an item of 16 query rows per key/value head streams the cache once per item, so a
 // sequence of more rows reads it several times; from there on the tensor-core tiles of 256 rows win.
-bool chunk_route(int64_t max_seqlen_q, int64_t G) { return max_seqlen_q * G > sage::kDecRows; }
+bool chunk_route(int64_t max_seqlen_q, int64_t G) { return max_seqlen_q * G > sage::kDecMaxRows; }
 
 // Tensor map of the packed queries: boxes of Gp heads by TT tokens by 64 channels.
 int query_map(CUtensorMap* map, const void* q, int dtype, int64_t D, int64_t heads, int64_t tokens, int64_t sh, int64_t st,
@@ -231,15 +231,17 @@ int launch_chunk(const PagedMaps& m, const sage::ChunkParams& p, cudaStream_t st
                       sage::kJoinRows * D / 4, 0, st, p.d);
 }
 
-template <int D, bool I8, typename T>
+template <int D, bool I8, typename T, int NR>
 int launch_decode(const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
-  using C = sage::DecodeCfg<D, I8>;
-  auto kern = sage::paged_decode_kernel<D, I8, T>;
+  using C = sage::DecodeCfg<D, I8, NR>;
+  auto kern = sage::paged_decode_kernel<D, I8, T, NR>;
+  constexpr int pieces = C::CTAS * 148;
+  static_assert(pieces <= sage::kDecMaxPieces && C::ROWS <= sage::kDecMaxRows, "workspace");
   if (int rc = ensure_smem(reinterpret_cast<const void*>(kern), C::SMEM)) return rc;
-  kern<<<sage::kDecPieces, sage::kDecThreads, C::SMEM, st>>>(m.k, m.v, m.ks, m.vs, p);
+  kern<<<pieces, sage::kDecThreads, C::SMEM, st>>>(m.k, m.v, m.ks, m.vs, p);
   SAGE_CUDA_TRY(cudaGetLastError());
-  return launch_early(sage::paged_combine_kernel<D, I8, T>,
-                      dim3(sage::kDecPieces, (unsigned)max_rows), sage::kCombineThreads, 0, st, p);
+  return launch_early(sage::paged_combine_kernel<D, I8, T, NR>, dim3(pieces, (unsigned)std::min(max_rows, C::ROWS)),
+                      sage::kCombineThreads, 0, st, p);
 }
 
 template <int D>
@@ -248,12 +250,15 @@ int chunk_dispatch(bool i8, bool bf, const PagedMaps& m, const sage::ChunkParams
   return bf ? launch_chunk<D, false, __nv_bfloat16>(m, p, st) : launch_chunk<D, false, __half>(m, p, st);
 }
 
+// Eight query rows where no sequence has more, else sixteen.
+template <int D, bool I8, typename T>
+int decode_rows(const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
+  return max_rows <= 8 ? launch_decode<D, I8, T, 1>(m, p, max_rows, st) : launch_decode<D, I8, T, 2>(m, p, max_rows, st);
+}
 template <int D>
 int decode_dispatch(bool i8, bool bf, const PagedMaps& m, const sage::DecodeParams& p, int max_rows, cudaStream_t st) {
-  if (i8) return bf ? launch_decode<D, true, __nv_bfloat16>(m, p, max_rows, st)
-                    : launch_decode<D, true, __half>(m, p, max_rows, st);
-  return bf ? launch_decode<D, false, __nv_bfloat16>(m, p, max_rows, st)
-            : launch_decode<D, false, __half>(m, p, max_rows, st);
+  if (i8) return bf ? decode_rows<D, true, __nv_bfloat16>(m, p, max_rows, st) : decode_rows<D, true, __half>(m, p, max_rows, st);
+  return bf ? decode_rows<D, false, __nv_bfloat16>(m, p, max_rows, st) : decode_rows<D, false, __half>(m, p, max_rows, st);
 }
 
 }  // namespace
@@ -365,12 +370,12 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   }
   m.ks = m.k;
   m.vs = m.v;
-  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, sage::kDecRows);
+  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, sage::kDecMaxRows);
   if (i8) {
     if (int rc = scale_map(&m.ks, c, false, tile)) return rc;
     if (int rc = scale_map(&m.vs, c, true, tile)) return rc;
   }
-  const size_t rows = size_t(2) * sage::kDecPieces * sage::kDecRows;
+  const size_t rows = size_t(2) * sage::kDecMaxPieces * sage::kDecMaxRows;
   p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
   p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
   return D == 128 ? decode_dispatch<128>(i8, bf, m, p, max_rows, st) : decode_dispatch<64>(i8, bf, m, p, max_rows, st);

@@ -321,7 +321,6 @@ __device__ __forceinline__ void codes_to_half16(const uint4& w, uint4& a, uint4&
   z = make_uint4(biased_to_half2(__byte_perm(u, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(u, 0x64646464u, 0x4342)),
                  biased_to_half2(__byte_perm(v, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(v, 0x64646464u, 0x4342)));
 }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
 
 template <int D, bool I8, typename T>
 __global__ void __launch_bounds__(kChunkThreads, 1)

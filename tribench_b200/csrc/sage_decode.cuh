@@ -5,11 +5,13 @@
 // visible keys, o = sum_j softmax(s)_j V_j. Key j < L is visible to the query at position p when
 // j <= p (causal) and, with a window W, j > p - W or j < sinks. A row that sees nothing gives 0.
 //
-// What bounds it: the cache is read once, so HBM (16-bit: 4 D bytes per key and head, INT8: 2 D + 8);
-// the products are 16-row mma.sync tiles, whose rate no shape here comes near to needing
-// (a 128-row tcgen05 tile would be almost all padding).
+// What bounds it: the cache is read once, so HBM (16-bit: 4 D bytes per key and head, INT8: 2 D + 8),
+// and for INT8, at half the bytes, the issue slots of widening the codes. The products are
+// mma.sync.m16n8k16 with the keys as the 16-row side: S^T = K Q^T and O^T = V^T P^T, so that 8 query
+// rows fill a product and the softmax holds 4 scores per lane and 16 keys (a tcgen05 tile's 128 rows
+// would be almost all padding). P^T changes sides by movmatrix.
 //
-// Work split. The unit is a tile of 64 keys of one (sequence, head, 16-row query tile) item. All
+// Work split. The unit is a tile of 64 keys of one (sequence, head, tile of 8 NR query rows) item. All
 // tiles of the call, in that order, form one line, cut into equal pieces, one per CTA: every CTA
 // streams the same number of tiles whatever the lengths are, and the host needs to know none of
 // them. A piece that holds an item whole writes its output; an item cut between pieces leaves
@@ -19,13 +21,18 @@
 // CTA: four consumer warps and a producer warp that loads tiles by TMA (one box per page and
 // operand) through a ring of stages. Each consumer warp owns 16 of a tile's 64 keys, with its own
 // running maximum, sum and output accumulators (registers); the four are joined once per item. K and
-// V fragments come from the swizzled tiles by ldmatrix (16-bit), or as plain byte loads converted in
-// registers (INT8: the codes are exact in fp16).
+// V fragments come from the swizzled tiles by ldmatrix (16-bit), or as plain byte loads widened in
+// registers (INT8).
 //
-// INT8: scores are (q . code) * k_scale; the weights of V's codes are p_j v_scale_j, kept relative to
-// their own running maximum, since v_scale may be anything while fp16 may not. bf16 queries are
-// brought to fp16 by a power of two per row: 8 significant bits fit into 11, and what falls below
-// 2^-24 of the row's largest value is lost far under bf16's own rounding.
+// The maximum is lazy: it moves, and the outputs are rescaled, only when a score exceeds it by more
+// than 2^8, so most tiles need no reduction over lanes; P <= 2^8 is kept in 16 bits, sums in fp32.
+//
+// INT8. K: byte c + 128 zero-extended is the fp16 subnormal (c + 128) 2^-24, exact, without an
+// instruction beyond the byte permutation; the scores become 2^24 S' - 128 sum(q), then times k_scale.
+// V: codes as exact fp16 values; its weights are p_j v_scale_j 2^-E, E following the largest v_scale
+// seen (raised when one exceeds it by 2^5). bf16 queries are brought to fp16 by a power of two per
+// row: 8 significant bits fit into 11, and what falls below 2^-24 of the row's largest value is lost
+// far under bf16's own rounding.
 #pragma once
 
 #include <type_traits>
@@ -38,8 +45,8 @@ namespace sage {
 constexpr int kDecWarps = 4;                         // consumer warps
 constexpr int kDecThreads = 32 * (kDecWarps + 1);    // + the producer warp
 constexpr int kDecKeys = 64;                         // keys per tile
-constexpr int kDecRows = 16;                         // query rows per item
-constexpr int kDecPieces = 2 * 148;                  // CTAs: two per SM
+constexpr int kDecMaxRows = 16;                      // query rows per item, at most: 8 NR
+constexpr int kDecMaxPieces = 3 * 148;               // CTAs, at most
 
 struct DecodeParams {
   PagedSeqs s;
@@ -50,8 +57,8 @@ struct DecodeParams {
   int page_shift;
   int causal, window, sinks;       // window 0: none
   float scale_log2;                // sm_scale * log2(e)
-  float* part;                     // [2 * CTAs][16][D] unnormalised outputs
-  float* part_ml;                  // [2 * CTAs][16][4]: max of scores, sum, max of weights
+  float* part;                     // [2 * CTAs][rows][D] unnormalised outputs
+  float* part_ml;                  // [2 * CTAs][rows][4]: max of scores, sum, unit of the outputs (log2)
   int4* desc;                      // [CTAs]: the item that a CTA's piece begins and does not end (sequence,
                                    // head, query tile or block, pieces that follow with its rest; 0: none)
   // Rows of the chunk kernel's blocks: parts of a head group (1 up to 128 heads), query heads of a
@@ -60,8 +67,9 @@ struct DecodeParams {
   unsigned long long wait_limit_ns;
 };
 
-template <int D, bool I8>
+template <int D, bool I8, int NR>
 struct DecodeCfg {
+  static constexpr int ROWS = 8 * NR;
   static constexpr int ELT = I8 ? 1 : 2;
   static constexpr int ROW_BYTES = D * ELT;
   static constexpr int ATOMS = ROW_BYTES > 128 ? 2 : 1;            // 128-byte column atoms per row
@@ -69,14 +77,16 @@ struct DecodeCfg {
   static constexpr int TILE = kDecKeys * ROW_BYTES;                // K (or V) bytes of a stage
   static constexpr int SCALES = I8 ? 512 : 0;                      // scale bytes of a stage, K or V
   static constexpr int STAGE = 2 * TILE + 2 * SCALES;
-  // Ring: 64 KB in flight per CTA, two CTAs per SM (what HBM needs in flight is about 45 KB per SM)
-  static constexpr int NS = 65536 / (2 * TILE) > 6 ? 6 : 65536 / (2 * TILE);
-  static constexpr int RED_STRIDE = D + 8;                         // floats per row: bank spread
+  // CTAs per SM: HBM needs about 45 KB in flight per SM; INT8 also wants warps to issue from
+  static constexpr int CTAS = (I8 && NR == 1) ? 3 : 2;
+  static constexpr int NS = I8 ? (D == 128 ? 3 : 6) : (D == 128 ? 2 : 4);
+  static constexpr int RED_STRIDE = D + 4;                         // floats per row: bank spread
   static constexpr int OFF_RED = NS * STAGE;
-  static constexpr int OFF_ML = OFF_RED + kDecWarps * kDecRows * RED_STRIDE * 4;
-  static constexpr int OFF_BAR = OFF_ML + kDecWarps * kDecRows * 4 * 4;
+  static constexpr int OFF_ML = OFF_RED + kDecWarps * ROWS * RED_STRIDE * 4;
+  static constexpr int OFF_BAR = OFF_ML + kDecWarps * ROWS * 4 * 4;
   static constexpr int OFF_MISC = OFF_BAR + 2 * NS * 8;
   static constexpr int SMEM = 1024 + OFF_MISC + 64;
+  static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
 // Key tiles of one sequence that some query of it sees: the sinks' tiles, then the rest.
@@ -97,10 +107,11 @@ __device__ __forceinline__ TileSpan tile_span(const PagedSeq& q, int window, int
 }
 __device__ __forceinline__ int tile_at(const TileSpan& t, int i) { return i < t.ns ? i : t.tw + i - t.ns; }
 
+template <int ROWS>
 __device__ __forceinline__ int64_t decode_tiles(const DecodeParams& p, int b) {
   const PagedSeq sq = paged_seq(p.s, b);
   const TileSpan ts = tile_span(sq, p.window, p.sinks, kDecKeys);
-  return (int64_t)p.Hkv * ((sq.n * (int64_t)p.G + kDecRows - 1) / kDecRows) * ts.count;
+  return (int64_t)p.Hkv * ((sq.n * (int64_t)p.G + ROWS - 1) / ROWS) * ts.count;
 }
 
 __device__ __forceinline__ void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -139,16 +150,26 @@ __device__ __forceinline__ uint32_t biased_to_half2(uint32_t bits) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// T: element type of q, o and a 16-bit cache.
-template <int D, bool I8, typename T>
-__global__ void __launch_bounds__(kDecThreads, 2)
+// Transpose of an 8 x 8 matrix of 16-bit values held as mma fragments.
+__device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+__device__ __forceinline__ int exponent(float x) { return min(max((int)((__float_as_uint(x) >> 23) & 255) - 127, -126), 120); }
+
+// T: element type of q, o and a 16-bit cache. NR: query rows of an item / 8.
+template <int D, bool I8, typename T, int NR>
+__global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
                         const DecodeParams p) {
-  using C = DecodeCfg<D, I8>;
+  using C = DecodeCfg<D, I8, NR>;
   using M = typename std::conditional<I8, __half, T>::type;  // operand type of the products
   constexpr int KS = D / 16;   // k-steps of q . K
-  constexpr int NT = D / 8;    // 8-column tiles of the output
+  constexpr int NT = D / 16;   // 16-channel tiles of the output
+  constexpr float LAZY = 8.0f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -172,7 +193,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   const int run = (p.s.batch + kDecThreads - 1) / kDecThreads;
   const int b_lo = min(p.s.batch, (int)threadIdx.x * run), b_hi = min(p.s.batch, b_lo + run);
   int64_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += decode_tiles(p, b);
+  for (int b = b_lo; b < b_hi; ++b) mine += decode_tiles<C::ROWS>(p, b);
   int64_t incl = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -198,7 +219,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     int64_t at = before + incl - mine;
     int b = b_lo;
     for (; b < b_hi - 1; ++b) {
-      const int64_t t = decode_tiles(p, b);
+      const int64_t t = decode_tiles<C::ROWS>(p, b);
       if (begin < at + t) break;
       at += t;
     }
@@ -227,7 +248,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     while (left > 0 && ok && b < p.s.batch) {
       const PagedSeq sq = paged_seq(p.s, b);
       const TileSpan ts = tile_span(sq, p.window, p.sinks, kDecKeys);
-      const int nmt = (sq.n * p.G + kDecRows - 1) / kDecRows;
+      const int nmt = (sq.n * p.G + C::ROWS - 1) / C::ROWS;
       const int64_t all = (int64_t)p.Hkv * nmt * ts.count;
       if (rem >= all) { rem = 0; ++b; continue; }  // the next sequence with tiles
       const int item = (int)(rem / ts.count), t0 = (int)(rem - (int64_t)item * ts.count);
@@ -297,98 +318,111 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   while (left > 0 && b < p.s.batch) {
     const PagedSeq sq = paged_seq(p.s, b);
     const TileSpan ts = tile_span(sq, p.window, p.sinks, kDecKeys);
-    const int nmt = (sq.n * p.G + kDecRows - 1) / kDecRows;
+    const int nmt = (sq.n * p.G + C::ROWS - 1) / C::ROWS;
     const int64_t all = (int64_t)p.Hkv * nmt * ts.count;
     if (rem >= all) { rem = 0; ++b; continue; }
     const int item = (int)(rem / ts.count), t0 = (int)(rem - (int64_t)item * ts.count);
     const int h = item / nmt, mt = item - h * nmt;
     const int n = (int)min((int64_t)(ts.count - t0), left);
-    const int rows = min(kDecRows, sq.n * p.G - mt * kDecRows);  // valid rows of the item
-    const int first = sq.len - sq.n;                            // position of the first new token
-    // this thread's two rows: token and keys [lo, hi) (and [0, sinks)) that it sees
-    int lo[2], hi[2];
-    const T* qp[2];
+    const int rows = min(C::ROWS, sq.n * p.G - mt * C::ROWS);  // valid rows of the item
+    const int first = sq.len - sq.n;                           // position of the first new token
+    // This thread's query rows 8 nt + 2 t, 8 nt + 2 t + 1: the keys [lo, hi) (and [0, sinks)) that they see
+    int lo[NR][2], hi[NR][2];
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int row = g + 8 * r, fr = mt * kDecRows + min(row, rows - 1);
-      const int tok = fr / p.G, hd = fr - tok * p.G;
-      const int pos = first + tok;
-      hi[r] = p.causal ? pos + 1 : sq.len;
-      lo[r] = p.window ? pos - p.window + 1 : 0;
-      qp[r] = row < rows ? static_cast<const T*>(p.q) + (int64_t)(sq.base + tok) * p.q_st +
-                               (int64_t)(h * p.G + hd) * p.q_sh
-                         : nullptr;
-    }
+    for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int pos = first + (mt * C::ROWS + min(8 * nt + 2 * t + c, rows - 1)) / p.G;
+        hi[nt][c] = p.causal ? pos + 1 : sq.len;
+        lo[nt][c] = p.window ? pos - p.window + 1 : 0;
+      }
     // bounds over all rows of the item: keys no row sees, and tiles that every row sees whole
-    const int tok_a = mt * kDecRows / p.G, tok_b = (mt * kDecRows + rows - 1) / p.G;
+    const int tok_a = mt * C::ROWS / p.G, tok_b = (mt * C::ROWS + rows - 1) / p.G;
     const int any_hi = p.causal ? first + tok_b + 1 : sq.len, all_hi = p.causal ? first + tok_a + 1 : sq.len;
     const int any_lo = p.window ? first + tok_a - p.window + 1 : 0, all_lo = p.window ? first + tok_b - p.window + 1 : 0;
 
-    // Q fragments. 16-bit: k index = channel. INT8: lane column t holds channels [t D/4, (t+1) D/4),
-    // k-step s its channels 4 s .. 4 s + 3, so that a K row's codes are contiguous per lane.
-    uint32_t qf[KS][4];
-    float qscale[2] = {p.scale_log2, p.scale_log2};
+    // Q fragments: row 8 nt + g. 16-bit: k index = channel. INT8: lane column t holds channels
+    // [t D/4, (t + 1) D/4), k-step s its channels 4 s .. 4 s + 3, so that a K row's codes are contiguous
+    // per lane.
+    uint32_t qf[NR][KS][2];
+    float qa[NR][2], qb[NR][2];  // score = qa S + qb, of this thread's rows 2 t, 2 t + 1
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
+    for (int nt = 0; nt < NR; ++nt) {
+      const int row = 8 * nt + g, fr = mt * C::ROWS + row, tok = fr / p.G, hd = fr - tok * p.G;
+      const bool in = row < rows;
+      const T* qp = static_cast<const T*>(p.q) + (in ? (int64_t)(sq.base + tok) * p.q_st + (int64_t)(h * p.G + hd) * p.q_sh : 0);
       if constexpr (!I8) {
 #pragma unroll
         for (int s = 0; s < KS; ++s)
 #pragma unroll
           for (int half = 0; half < 2; ++half)
-            qf[s][half * 2 + r] =
-                qp[r] ? *reinterpret_cast<const uint32_t*>(qp[r] + s * 16 + half * 8 + t * 2) : 0u;
+            qf[nt][s][half] = in ? *reinterpret_cast<const uint32_t*>(qp + s * 16 + half * 8 + t * 2) : 0u;
+        qa[nt][0] = qa[nt][1] = p.scale_log2;
+        qb[nt][0] = qb[nt][1] = 0.0f;
       } else {
+        float unit = 1.0f, sum = 0.0f;
         uint4 raw[D / 32];
+        uint32_t m = 0;
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-          raw[x] = qp[r] ? ldg_nc_v4(qp[r] + t * (D / 4) + x * 8) : make_uint4(0u, 0u, 0u, 0u);
-        if constexpr (std::is_same<T, __half>::value) {
+        for (int x = 0; x < D / 32; ++x) {
+          raw[x] = in ? ldg_nc_v4(qp + t * (D / 4) + x * 8) : make_uint4(0u, 0u, 0u, 0u);
+          if constexpr (!std::is_same<T, __half>::value) {
+            float f[8];
+            Half8<T>::to_float(raw[x], f);
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            qf[2 * x][r] = raw[x].x;
-            qf[2 * x][2 + r] = raw[x].y;
-            qf[2 * x + 1][r] = raw[x].z;
-            qf[2 * x + 1][2 + r] = raw[x].w;
+            for (int y = 0; y < 8; ++y) m = max(m, abs_bits(f[y]));
           }
-        } else {
-          float f[D / 4];
-          float m = 0.0f;
+        }
+        if constexpr (!std::is_same<T, __half>::value) {
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+          m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+          unit = pow2(exponent(__uint_as_float(m)));
+        }
+        const float down = 1.0f / unit;  // a power of two: exact
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            float e[8];
-            Half8<T>::to_float(raw[x], e);
+        for (int x = 0; x < D / 32; ++x) {
+          float f[8];
+          Half8<T>::to_float(raw[x], f);
+          if constexpr (!std::is_same<T, __half>::value) {
 #pragma unroll
-            for (int y = 0; y < 8; ++y) {
-              f[x * 8 + y] = e[y];
-              m = fmaxf(m, fabsf(e[y]));
-            }
+            for (int y = 0; y < 8; ++y) f[y] *= down;
+            raw[x] = Half8<__half>::from_float(f);
+            Half8<__half>::to_float(raw[x], f);
           }
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-          m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-          // 2^e <= m < 2^(e+1): multiply by 2^-e, and the scores by 2^e (two factors: e may be -126)
-          const int e = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 126);
-          const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-          qscale[r] *= __uint_as_float((uint32_t)(127 + e) << 23);
+          sum += ((f[0] + f[1]) + (f[2] + f[3])) + ((f[4] + f[5]) + (f[6] + f[7]));
+          qf[nt][2 * x][0] = raw[x].x;
+          qf[nt][2 * x][1] = raw[x].y;
+          qf[nt][2 * x + 1][0] = raw[x].z;
+          qf[nt][2 * x + 1][1] = raw[x].w;
+        }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        const float a = p.scale_log2 * unit;
 #pragma unroll
-          for (int x = 0; x < D / 32; ++x) {
-            const float* y = f + x * 8;
-            qf[2 * x][r] = pack2<__half>(y[0] * down, y[1] * down);
-            qf[2 * x][2 + r] = pack2<__half>(y[2] * down, y[3] * down);
-            qf[2 * x + 1][r] = pack2<__half>(y[4] * down, y[5] * down);
-            qf[2 * x + 1][2 + r] = pack2<__half>(y[6] * down, y[7] * down);
-          }
+        for (int c = 0; c < 2; ++c) {  // row 2 t + c is that of lanes 4 (2 t + c)
+          const float ar = __shfl_sync(0xffffffffu, a, 4 * (2 * t + c)), sr = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + c));
+          qa[nt][c] = ar * 16777216.0f;
+          qb[nt][c] = -128.0f * sr * ar;
         }
       }
     }
 
-    float acc[NT][4];
+    float acc[NT][NR][4];
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][c] = 0.0f;
-    float m1[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-    float m2[2] = {-INFINITY, -INFINITY};  // INT8: maximum of score + log2(v_scale)
+      for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[i][nt][c] = 0.0f;
+    float m1[NR][2], l[NR][2];  // l: this lane's part
+#pragma unroll
+    for (int nt = 0; nt < NR; ++nt) {
+      m1[nt][0] = m1[nt][1] = -INFINITY;
+      l[nt][0] = l[nt][1] = 0.0f;
+    }
+    int unit_v = -126;  // INT8: weights are in units of 2^unit_v
 
+#pragma unroll 1
     for (int i = t0; i < t0 + n; ++i, ++it) {
       const int s = it % C::NS;
       if (ok) ok = mbar_wait(full + s, (it / C::NS) & 1, abort_flag, 4, p.wait_limit_ns);
@@ -397,136 +431,168 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       const uint32_t kt = smem_base + s * C::STAGE, vt = kt + C::TILE;
       const int key0 = tile_at(ts, i) * kDecKeys;
       const int k_warp = warp * 16;  // this warp's keys of the tile
-      // ---- scores of 16 rows x 16 keys
-      float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
-      float lv[2][2] = {{0.f, 0.f}, {0.f, 0.f}};  // INT8: log2(v_scale) of this thread's keys
+      // ---- scores of 16 keys x 8 NR rows; this lane: keys g, g + 8
+      float sc[NR][4];
+#pragma unroll
+      for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) sc[nt][c] = 0.0f;
+      float vs[2] = {1.0f, 1.0f};
+      if constexpr (!I8) {
+        const int r = lane & 7, mi = lane >> 3;
+        const int key = k_warp + (mi & 1) * 8 + r;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const int chunk = 2 * ks + (mi >> 1);
+          uint32_t a[4];
+          ldmatrix_x4(a, kt + (chunk >> 3) * (kDecKeys * 128) + key * 128 + (((chunk & 7) ^ r) << 4));
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt) mma16816<M>(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[nt][c] *= qa[nt][c & 1];
+      } else {
+        uint32_t w[2][D / 16];
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int key = k_warp + x * 8 + g;
+#pragma unroll
+          for (int y = 0; y < D / 64; ++y) {
+            const int chunk = t * (D / 64) + y;
+            const int sw = D == 128 ? (chunk ^ (key & 7)) : (chunk ^ ((key >> 1) & 3));
+            const uint4 v = *reinterpret_cast<const uint4*>(smem + s * C::STAGE + key * D + sw * 16);
+            w[x][4 * y] = v.x; w[x][4 * y + 1] = v.y; w[x][4 * y + 2] = v.z; w[x][4 * y + 3] = v.w;
+          }
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+          const uint32_t u0 = w[0][ks] ^ 0x80808080u, u1 = w[1][ks] ^ 0x80808080u;
+          const uint32_t a[4] = {__byte_perm(u0, 0u, 0x4140), __byte_perm(u1, 0u, 0x4140), __byte_perm(u0, 0u, 0x4342),
+                                 __byte_perm(u1, 0u, 0x4342)};
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt) mma16816<M>(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
+        }
+        // a page's scales start on 128 bytes
+        const int kk = k_warp + g, sh = min(p.page_shift, 6), in_page = (1 << sh) - 1, pitch = max(32, 1 << sh);
+        const float* scales = reinterpret_cast<const float*>(smem + s * C::STAGE + 2 * C::TILE);
+        const int at = (kk >> sh) * pitch + (kk & in_page);  // pages hold multiples of 16 keys: key g + 8 is in the same one
+        const float ks0 = scales[at], ks1 = scales[at + 8];
+        vs[0] = scales[C::SCALES / 4 + at];
+        vs[1] = scales[C::SCALES / 4 + at + 8];
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) sc[nt][c] = fmaf(sc[nt][c], qa[nt][c & 1], qb[nt][c & 1]) * (c < 2 ? ks0 : ks1);
+      }
+      // ---- mask
+      const bool whole = key0 + kDecKeys <= all_hi && (key0 >= all_lo || key0 + kDecKeys <= p.sinks);
+      uint32_t vm[2] = {0xffffffffu, 0xffffffffu};  // 16-bit: V rows 2 t (+ 1), + 8 that some query sees
+      uint32_t seen = 0xffffffffu;                  // bit 4 nt + c
+      if (!whole) {
+        seen = 0;
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int key = key0 + k_warp + (c >> 1) * 8 + g;
+            const bool see = key < hi[nt][c & 1] && (key >= lo[nt][c & 1] || key < p.sinks);
+            if (!see) sc[nt][c] = -INFINITY;
+            seen |= see ? 1u << (4 * nt + c) : 0u;
+          }
+        if constexpr (!I8) {
+          // rows that no query sees may hold anything (an unused page's NaN): 0 instead, as their weight is
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            const int key = key0 + k_warp + x * 8 + 2 * t;
+            const bool a = key < any_hi && (key >= any_lo || key < p.sinks);
+            const bool z = key + 1 < any_hi && (key + 1 >= any_lo || key + 1 < p.sinks);
+            vm[x] = (a ? 0xffffu : 0u) | (z ? 0xffff0000u : 0u);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {  // nor may an unused scale raise the unit
+            const int key = key0 + k_warp + x * 8 + g;
+            if (!(key < any_hi && (key >= any_lo || key < p.sinks))) vs[x] = 0.0f;
+          }
+        }
+      }
+      // ---- the maximum (and INT8's unit), where a score outgrew it
+      float down = 1.0f;
+      if constexpr (I8) down = pow2(-unit_v);
+      bool grow = I8 && fmaxf(vs[0], vs[1]) * down > 32.0f;
+#pragma unroll
+      for (int nt = 0; nt < NR; ++nt)
+        grow |= fmaxf(sc[nt][0], sc[nt][2]) > m1[nt][0] + LAZY || fmaxf(sc[nt][1], sc[nt][3]) > m1[nt][1] + LAZY;
+      if (__any_sync(0xffffffffu, grow)) {
+        float shrink = 1.0f;
+        if constexpr (I8) {
+          float mv = fmaxf(fmaxf(vs[0], vs[1]), 0.0f);
+#pragma unroll
+          for (int o = 4; o < 32; o <<= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
+          const int e = max(unit_v, exponent(mv));
+          shrink = pow2(max(unit_v - e, -126));
+          unit_v = e;
+          down = pow2(-e);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float mn = fmaxf(m1[nt][c], mx);
+            const float alpha = mn == -INFINITY ? 1.0f : ex2_approx(m1[nt][c] - mn);
+            m1[nt][c] = mn;
+            l[nt][c] *= alpha;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              acc[x][nt][c] *= alpha * shrink;
+              acc[x][nt][c + 2] *= alpha * shrink;
+            }
+          }
+      }
+      // ---- weights, as the B operand of O^T = V^T P^T
+      uint32_t pf[NR][2];
+      if constexpr (I8) {
+        vs[0] *= down;
+        vs[1] *= down;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NR; ++nt) {
+        const float u0 = m1[nt][0] == -INFINITY ? 0.0f : m1[nt][0], u1 = m1[nt][1] == -INFINITY ? 0.0f : m1[nt][1];
+        float e[4] = {ex2_approx(sc[nt][0] - u0), ex2_approx(sc[nt][1] - u1), ex2_approx(sc[nt][2] - u0),
+                      ex2_approx(sc[nt][3] - u1)};
+        l[nt][0] += e[0] + e[2];
+        l[nt][1] += e[1] + e[3];
+        if constexpr (I8) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            e[c] *= vs[c >> 1];
+            if (!whole && !((seen >> (4 * nt + c)) & 1u)) e[c] = 0.0f;  // the scale may be a NaN
+          }
+        }
+        pf[nt][0] = movmatrix(pack2<M>(e[0], e[1]));
+        pf[nt][1] = movmatrix(pack2<M>(e[2], e[3]));
+      }
+      // ---- O^T += V^T P^T over this warp's 16 keys
       if constexpr (!I8) {
         const int r = lane & 7, mi = lane >> 3;
         const int key = k_warp + (mi >> 1) * 8 + r;
 #pragma unroll
-        for (int ks = 0; ks < KS; ++ks) {
-          const int chunk = 2 * ks + (mi & 1);
-          uint32_t bf[4];
-          ldmatrix_x4(bf, kt + (chunk >> 3) * (kDecKeys * 128) + key * 128 + (((chunk & 7) ^ r) << 4));
-          mma16816<M>(sc[0], qf[ks], bf[0], bf[1]);
-          mma16816<M>(sc[1], qf[ks], bf[2], bf[3]);
+        for (int j = 0; j < NT; ++j) {
+          const int chunk = 2 * j + (mi & 1);
+          uint32_t a[4];
+          ldmatrix_x4_trans(a, vt + (chunk >> 3) * (kDecKeys * 128) + key * 128 + (((chunk & 7) ^ r) << 4));
+          a[0] &= vm[0]; a[1] &= vm[0]; a[2] &= vm[1]; a[3] &= vm[1];
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt) mma16816<M>(acc[j][nt], a, pf[nt][0], pf[nt][1]);
         }
       } else {
-        const float* kscale = reinterpret_cast<const float*>(smem + s * C::STAGE + 2 * C::TILE);
-        const float* vscale = kscale + C::SCALES / 4;
-        float ksc[2][2];
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-          const int key = k_warp + nt * 8 + g;
-          uint32_t w[D / 16];
-#pragma unroll
-          for (int x = 0; x < D / 64; ++x) {
-            const int chunk = t * (D / 64) + x;
-            const int sw = D == 128 ? (chunk ^ (key & 7)) : (chunk ^ ((key >> 1) & 3));
-            const uint4 v = *reinterpret_cast<const uint4*>(smem + s * C::STAGE + key * D + sw * 16);
-            w[4 * x] = v.x; w[4 * x + 1] = v.y; w[4 * x + 2] = v.z; w[4 * x + 3] = v.w;
-          }
-#pragma unroll
-          for (int ks = 0; ks < KS; ++ks) {
-            const uint32_t u = w[ks] ^ 0x80808080u;
-            mma16816<M>(sc[nt], qf[ks], biased_to_half2(__byte_perm(u, 0x64646464u, 0x4140)),
-                        biased_to_half2(__byte_perm(u, 0x64646464u, 0x4342)));
-          }
-          // a page's scales start on 128 bytes
-          const int kk = k_warp + nt * 8 + 2 * t;
-          const int sh = min(p.page_shift, 6);
-          const int at = (kk >> sh) * (sh < 5 ? 32 : (1 << sh)) + (kk & ((1 << sh) - 1));
-          const float2 k2 = *reinterpret_cast<const float2*>(kscale + at);
-          const float2 v2 = *reinterpret_cast<const float2*>(vscale + at);
-          ksc[nt][0] = k2.x; ksc[nt][1] = k2.y;
-          lv[nt][0] = __log2f(v2.x); lv[nt][1] = __log2f(v2.y);
-        }
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) sc[nt][c] *= ksc[nt][c & 1];
-      }
-      // ---- mask and softmax
-      const bool whole = key0 + kDecKeys <= all_hi && (key0 >= all_lo || key0 + kDecKeys <= p.sinks);
-      float w2[2][4];  // INT8: exponents of the weights
-#pragma unroll
-      for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int r = c >> 1, key = key0 + k_warp + nt * 8 + 2 * t + (c & 1);
-          const bool see = whole || (key < hi[r] && (key >= lo[r] || key < p.sinks));
-          const float x = sc[nt][c] * qscale[r];
-          sc[nt][c] = see ? x : -INFINITY;
-          if constexpr (I8) w2[nt][c] = see ? x + lv[nt][c & 1] : -INFINITY;
-        }
-      uint32_t pf[4];
-      float p_out[2][4];
-#pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        float mx = fmaxf(fmaxf(sc[0][2 * r], sc[0][2 * r + 1]), fmaxf(sc[1][2 * r], sc[1][2 * r + 1]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m1[r], mx), use = mn == -INFINITY ? 0.0f : mn;
-        const float alpha = ex2_approx(m1[r] - use);
-        m1[r] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            const float e = ex2_approx(sc[nt][2 * r + c] - use);
-            sum += e;
-            p_out[nt][2 * r + c] = e;
-          }
-        l[r] = fmaf(l[r], alpha, sum);
-        float beta = alpha;
-        if constexpr (I8) {
-          float my = fmaxf(fmaxf(w2[0][2 * r], w2[0][2 * r + 1]), fmaxf(w2[1][2 * r], w2[1][2 * r + 1]));
-          my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 1));
-          my = fmaxf(my, __shfl_xor_sync(0xffffffffu, my, 2));
-          const float wn = fmaxf(m2[r], my), uw = wn == -INFINITY ? 0.0f : wn;
-          beta = ex2_approx(m2[r] - uw);
-          m2[r] = wn;
-#pragma unroll
-          for (int nt = 0; nt < 2; ++nt)
-#pragma unroll
-            for (int c = 0; c < 2; ++c) p_out[nt][2 * r + c] = ex2_approx(w2[nt][2 * r + c] - uw);
-        }
-        if (__any_sync(0xffffffffu, beta != 1.0f)) {
-#pragma unroll
-          for (int x = 0; x < NT; ++x) {
-            acc[x][2 * r] *= beta;
-            acc[x][2 * r + 1] *= beta;
-          }
-        }
-      }
-      pf[0] = pack2<M>(p_out[0][0], p_out[0][1]);
-      pf[1] = pack2<M>(p_out[0][2], p_out[0][3]);
-      pf[2] = pack2<M>(p_out[1][0], p_out[1][1]);
-      pf[3] = pack2<M>(p_out[1][2], p_out[1][3]);
-      // ---- P . V over this warp's 16 keys
-      if constexpr (!I8) {
-        // rows that no query sees may hold anything (an unused page's NaN): 0 instead, as their weight is
-        uint32_t vm[2];
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int key = key0 + k_warp + x * 8 + 2 * t;
-          const bool a = whole || (key < any_hi && (key >= any_lo || key < p.sinks));
-          const bool z = whole || (key + 1 < any_hi && (key + 1 >= any_lo || key + 1 < p.sinks));
-          vm[x] = (a ? 0xffffu : 0u) | (z ? 0xffff0000u : 0u);
-        }
-        const int r = lane & 7, mi = lane >> 3;
-        const int key = k_warp + (mi & 1) * 8 + r;
-#pragma unroll
-        for (int j = 0; j < NT / 2; ++j) {
-          const int chunk = 2 * j + (mi >> 1);
-          uint32_t bf[4];
-          ldmatrix_x4_trans(bf, vt + (chunk >> 3) * (kDecKeys * 128) + key * 128 + (((chunk & 7) ^ r) << 4));
-          mma16816<M>(acc[2 * j], pf, bf[0] & vm[0], bf[1] & vm[1]);
-          mma16816<M>(acc[2 * j + 1], pf, bf[2] & vm[0], bf[3] & vm[1]);
-        }
-      } else {
-        // column n of output tile i is channel n D/8 + i: a lane's D/8 codes of a key are contiguous
+        // rows g and g + 8 of output tile i are channels g D/8 + 2 i and + 1: a lane's D/8 codes of a key
+        // are contiguous
         constexpr int W = D / 32;  // words of codes per key
         uint32_t w[4][W];
 #pragma unroll
@@ -546,88 +612,89 @@ __global__ void __launch_bounds__(kDecThreads, 2)
 #pragma unroll
         for (int y = 0; y < W; ++y) {
           // bytes of keys 2t, 2t + 1 interleaved, channel by channel; the same for 2t + 8, 2t + 9
-          const uint32_t a01 = __byte_perm(w[0][y], w[1][y], 0x5140), a23 = __byte_perm(w[0][y], w[1][y], 0x7362);
-          const uint32_t c01 = __byte_perm(w[2][y], w[3][y], 0x5140), c23 = __byte_perm(w[2][y], w[3][y], 0x7362);
-          mma16816<M>(acc[4 * y], pf, biased_to_half2(__byte_perm(a01, 0x64646464u, 0x4140)),
-                      biased_to_half2(__byte_perm(c01, 0x64646464u, 0x4140)));
-          mma16816<M>(acc[4 * y + 1], pf, biased_to_half2(__byte_perm(a01, 0x64646464u, 0x4342)),
-                      biased_to_half2(__byte_perm(c01, 0x64646464u, 0x4342)));
-          mma16816<M>(acc[4 * y + 2], pf, biased_to_half2(__byte_perm(a23, 0x64646464u, 0x4140)),
-                      biased_to_half2(__byte_perm(c23, 0x64646464u, 0x4140)));
-          mma16816<M>(acc[4 * y + 3], pf, biased_to_half2(__byte_perm(a23, 0x64646464u, 0x4342)),
-                      biased_to_half2(__byte_perm(c23, 0x64646464u, 0x4342)));
+          const uint32_t k01 = __byte_perm(w[0][y], w[1][y], 0x5140), k23 = __byte_perm(w[0][y], w[1][y], 0x7362);
+          const uint32_t n01 = __byte_perm(w[2][y], w[3][y], 0x5140), n23 = __byte_perm(w[2][y], w[3][y], 0x7362);
+          const uint32_t a[4] = {biased_to_half2(__byte_perm(k01, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(k01, 0x64646464u, 0x4342)),
+                                 biased_to_half2(__byte_perm(n01, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(n01, 0x64646464u, 0x4342))};
+          const uint32_t z[4] = {biased_to_half2(__byte_perm(k23, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(k23, 0x64646464u, 0x4342)),
+                                 biased_to_half2(__byte_perm(n23, 0x64646464u, 0x4140)), biased_to_half2(__byte_perm(n23, 0x64646464u, 0x4342))};
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt) {
+            mma16816<M>(acc[2 * y][nt], a, pf[nt][0], pf[nt][1]);
+            mma16816<M>(acc[2 * y + 1][nt], z, pf[nt][0], pf[nt][1]);
+          }
         }
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(empty + s);
     }
 
-    // ---- join the four warps
+    // ---- join the four warps: maxima, sums and units first
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-      l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-      if (t == 0) {
-        float* x = ml + (warp * kDecRows + g + 8 * r) * 4;
-        x[0] = m1[r];
-        x[1] = l[r];
-        x[2] = I8 ? m2[r] : m1[r];
+    for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[nt][c] += __shfl_xor_sync(0xffffffffu, l[nt][c], o);
+        if (g == 0) {
+          float* x = ml + (warp * C::ROWS + 8 * nt + 2 * t + c) * 4;
+          x[0] = m1[nt][c];
+          x[1] = l[nt][c];
+          x[2] = I8 ? m1[nt][c] + unit_v : m1[nt][c];
+        }
       }
-    }
     asm volatile("bar.sync 1, %0;" ::"n"(kDecWarps * 32) : "memory");
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      float mo = -INFINITY;
+    for (int nt = 0; nt < NR; ++nt)
 #pragma unroll
-      for (int w = 0; w < kDecWarps; ++w) mo = fmaxf(mo, ml[(w * kDecRows + g + 8 * r) * 4 + 2]);
-      const float f = ex2_approx((I8 ? m2[r] : m1[r]) - (mo == -INFINITY ? 0.0f : mo));
-      float* dst = red + (warp * kDecRows + g + 8 * r) * C::RED_STRIDE;
-      if constexpr (!I8) {
+      for (int c = 0; c < 2; ++c) {
+        const int row = 8 * nt + 2 * t + c;
+        float mo = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < NT; ++x)
-          *reinterpret_cast<float2*>(dst + x * 8 + 2 * t) = make_float2(acc[x][2 * r] * f, acc[x][2 * r + 1] * f);
-      } else {
+        for (int w = 0; w < kDecWarps; ++w) mo = fmaxf(mo, ml[(w * C::ROWS + row) * 4 + 2]);
+        const float f = ex2_approx((I8 ? m1[nt][c] + unit_v : m1[nt][c]) - (mo == -INFINITY ? 0.0f : mo));
+        float* dst = red + (warp * C::ROWS + row) * C::RED_STRIDE;
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int x = 0; x < NT; x += 4)
-            *reinterpret_cast<float4*>(dst + (2 * t + c) * (D / 8) + x) =
-                make_float4(acc[x][2 * r + c] * f, acc[x + 1][2 * r + c] * f, acc[x + 2][2 * r + c] * f,
-                            acc[x + 3][2 * r + c] * f);
+        for (int x = 0; x < NT; ++x) {
+          if constexpr (!I8) {
+            dst[16 * x + g] = acc[x][nt][c] * f;
+            dst[16 * x + g + 8] = acc[x][nt][c + 2] * f;
+          } else {
+            *reinterpret_cast<float2*>(dst + g * (D / 8) + 2 * x) = make_float2(acc[x][nt][c] * f, acc[x][nt][c + 2] * f);
+          }
+        }
       }
-    }
     asm volatile("bar.sync 1, %0;" ::"n"(kDecWarps * 32) : "memory");
     const bool begins = t0 == 0, ends = t0 + n == ts.count;
     const int slot = 2 * cta + (begins ? 1 : 0);
-#pragma unroll
-    for (int x = 0; x < kDecRows * (D / 4) / (kDecWarps * 32); ++x) {
-      const int idx = x * kDecWarps * 32 + threadIdx.x;
+#pragma unroll 1
+    for (int idx = threadIdx.x; idx < C::ROWS * (D / 4); idx += kDecWarps * 32) {
       const int row = idx / (D / 4), c4 = idx % (D / 4);
       if (row >= rows) continue;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       float ms = -INFINITY, mo = -INFINITY, sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
-        const float4 v = *reinterpret_cast<const float4*>(red + (w * kDecRows + row) * C::RED_STRIDE + c4 * 4);
+        const float4 v = *reinterpret_cast<const float4*>(red + (w * C::ROWS + row) * C::RED_STRIDE + c4 * 4);
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
-        ms = fmaxf(ms, ml[(w * kDecRows + row) * 4]);
-        mo = fmaxf(mo, ml[(w * kDecRows + row) * 4 + 2]);
+        ms = fmaxf(ms, ml[(w * C::ROWS + row) * 4]);
+        mo = fmaxf(mo, ml[(w * C::ROWS + row) * 4 + 2]);
       }
       const float use = ms == -INFINITY ? 0.0f : ms;
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
-        const float* y = ml + (w * kDecRows + row) * 4;
+        const float* y = ml + (w * C::ROWS + row) * 4;
         sum = fmaf(y[1], ex2_approx(y[0] - use), sum);
       }
       if (begins && ends) {
-        // INT8: the output is relative to the maximum of the weights, the sum to that of the scores
+        // INT8: the outputs' unit is their own
         const float inv = sum == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - use) / sum : 1.0f / sum);
-        const int fr = mt * kDecRows + row, tok = fr / p.G, hd = fr - tok * p.G;
+        const int fr = mt * C::ROWS + row, tok = fr / p.G, hd = fr - tok * p.G;
         T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(h * p.G + hd) * p.o_sh + c4 * 4;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
       } else {
-        *reinterpret_cast<float4*>(p.part + ((int64_t)slot * kDecRows + row) * D + c4 * 4) = o;
-        if (c4 == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * kDecRows + row) * 4) = make_float4(ms, sum, mo, 0.0f);
+        *reinterpret_cast<float4*>(p.part + ((int64_t)slot * C::ROWS + row) * D + c4 * 4) = o;
+        if (c4 == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * C::ROWS + row) * 4) = make_float4(ms, sum, mo, 0.0f);
       }
     }
     if (begins && !ends) cut = make_int4(b, h, mt, (int)((ts.count - n + per - 1) / per));
@@ -642,9 +709,9 @@ __global__ void __launch_bounds__(kDecThreads, 2)
 // (slot 2 c + 1) has its other parts in slots 2 c' of the pieces that follow. Block (c, row) joins one
 // row: eight warps share its parts, lanes hold D / 32 channels each.
 constexpr int kCombineThreads = 256;
-template <int D, bool I8, typename T>
+template <int D, bool I8, typename T, int NR>
 __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const DecodeParams p) {
-  constexpr int E = D / 32, W = kCombineThreads / 32;
+  constexpr int E = D / 32, W = kCombineThreads / 32, ROWS = 8 * NR;
   __shared__ float s_o[W][D];
   __shared__ float s_ml[W][3];
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -652,7 +719,7 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
   if (d.w == 0) return;
   const int warp = warp_id(), lane = lane_id(), row = blockIdx.y;
   const PagedSeq sq = paged_seq(p.s, d.x);
-  const int fr = d.z * kDecRows + row;
+  const int fr = d.z * ROWS + row;
   if (fr >= sq.n * p.G) return;
   const int tok = fr / p.G, hd = fr - tok * p.G;
   float o[E], ms = -INFINITY, l = 0.0f, mo = -INFINITY;
@@ -661,8 +728,8 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
 #pragma unroll 4
   for (int j = warp; j <= d.w; j += W) {
     const int64_t slot = j == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + j);
-    const float4 x = *reinterpret_cast<const float4*>(p.part_ml + (slot * kDecRows + row) * 4);
-    const float* src = p.part + (slot * kDecRows + row) * D + lane * E;
+    const float4 x = *reinterpret_cast<const float4*>(p.part_ml + (slot * ROWS + row) * 4);
+    const float* src = p.part + (slot * ROWS + row) * D + lane * E;
     float v[E];
     if constexpr (E == 4) {
       const float4 y = *reinterpret_cast<const float4*>(src);
