@@ -54,7 +54,9 @@ struct DecodeParams {
   void* o;
   int64_t q_st, q_sh, o_st, o_sh;  // element strides: token, head
   int Hkv, G;
-  int page_shift;
+  int page_shift, pages;
+  const float* k_scale;            // INT8: [pages][Hkv][page]
+  const float* v_scale;
   int causal, window, sinks;       // window 0: none
   float scale_log2;                // sm_scale * log2(e)
   float* part;                     // [2 * CTAs][rows][D] unnormalised outputs
@@ -75,8 +77,8 @@ struct DecodeCfg {
   static constexpr int ATOMS = ROW_BYTES > 128 ? 2 : 1;            // 128-byte column atoms per row
   static constexpr int BOX = ROW_BYTES > 128 ? 128 / ELT : D;      // TMA box width, elements
   static constexpr int TILE = kDecKeys * ROW_BYTES;                // K (or V) bytes of a stage
-  static constexpr int SCALES = I8 ? 512 : 0;                      // scale bytes of a stage, K or V
-  static constexpr int STAGE = 2 * TILE + 2 * SCALES;
+  static constexpr int SCALES = I8 ? 256 : 0;                      // scale bytes of a stage, K or V
+  static constexpr int STAGE = 2 * TILE + (I8 ? 1024 : 0);         // tiles start on 1024 bytes
   // CTAs per SM: HBM needs about 45 KB in flight per SM; INT8 also wants warps to issue from
   static constexpr int CTAS = (I8 && NR == 1) ? 3 : 2;
   static constexpr int NS = I8 ? (D == 128 ? 3 : 6) : (D == 128 ? 2 : 4);
@@ -133,6 +135,9 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t* a, uint3
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
+}
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -163,7 +168,6 @@ __device__ __forceinline__ int exponent(float x) { return min(max((int)((__float
 template <int D, bool I8, typename T, int NR>
 __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
-                        const __grid_constant__ CUtensorMap tmKs, const __grid_constant__ CUtensorMap tmVs,
                         const DecodeParams p) {
   using C = DecodeCfg<D, I8, NR>;
   using M = typename std::conditional<I8, __half, T>::type;  // operand type of the products
@@ -183,7 +187,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::NS; ++s) {
-      mbar_init(full + s, 1);
+      mbar_init(full + s, I8 ? 33 : 1);  // INT8: the producer's lanes bring four scales each
       mbar_init(empty + s, kDecWarps);
     }
     *abort_flag = 0;
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
     const int rows = min(page, kDecKeys);            // rows of a box
     const int ppt = kDecKeys / rows;                 // pages of a tile
     const int batch_tiles = 32 / ppt;                // tiles whose page numbers the 32 lanes hold
-    const int boxes = ppt * 2 * C::ATOMS + (I8 ? ppt * 2 : 0);
+    const int boxes = ppt * 2 * C::ATOMS;
     int it = 0;
     bool ok = true;
     while (left > 0 && ok && b < p.s.batch) {
@@ -275,22 +279,26 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
           }
           uint8_t* st = smem + s * C::STAGE;
           if (lane == 0)
-            mbar_arrive_expect_tx(full + s, 2 * C::TILE + (I8 ? 2 * kDecKeys * 4 : 0));
+            mbar_arrive_expect_tx(full + s, 2 * C::TILE);
           __syncwarp();
-          // box l: sub-page, then column atom, then K / V (then the scales)
+          // box l: sub-page, then column atom, then K / V
           const int sub = lane % ppt;
           const int id = __shfl_sync(0xffffffffu, ids, (i - i0) * ppt + sub);
           const int y = (tile_at(ts, i) * kDecKeys) & (page - 1);  // 0 where a tile holds whole pages
-          const int rest = lane / ppt;
-          if (lane < boxes) {
-            if (rest < 2 * C::ATOMS) {
-              const int atom = rest % C::ATOMS, isv = rest / C::ATOMS;
-              tma_load_4d(st + isv * C::TILE + atom * (kDecKeys * 128) + sub * rows * (C::ROW_BYTES > 128 ? 128 : C::ROW_BYTES),
-                          isv ? &tmV : &tmK, full + s, atom * C::BOX, y, h, id);
-            } else {
-              const int isv = rest - 2 * C::ATOMS;
-              tma_load_4d(st + 2 * C::TILE + isv * C::SCALES + sub * 128, isv ? &tmVs : &tmKs, full + s, y, h, id, 0);
-            }
+          const int rest = lane / ppt, atom = rest % C::ATOMS, isv = rest / C::ATOMS;
+          if (lane < boxes)
+            tma_load_4d(st + isv * C::TILE + atom * (kDecKeys * 128) + sub * rows * (C::ROW_BYTES > 128 ? 128 : C::ROW_BYTES),
+                        isv ? &tmV : &tmK, full + s, atom * C::BOX, y, h, id);
+          if constexpr (I8) {
+            // scales of keys 4 x .. 4 x + 3, K's from lanes 0-15, V's from 16-31: a copy of 16 bytes
+            // each costs less than a box per page
+            const int x = (lane & 15) * 4, sv = lane >> 4;
+            const int pg = __shfl_sync(0xffffffffu, ids, (i - i0) * ppt + x / rows);
+            const bool in = pg >= 0 && pg < p.pages;
+            const float* src = (sv ? p.v_scale : p.k_scale) +
+                               (in ? ((((int64_t)pg * p.Hkv + h) << p.page_shift) + ((y + x) & (page - 1))) : 0);
+            cp_async16(smem_u32(st + 2 * C::TILE + sv * C::SCALES) + x * 4, src, in);
+            asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(full + s)) : "memory");
           }
         }
       }
@@ -474,10 +482,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
 #pragma unroll
           for (int nt = 0; nt < NR; ++nt) mma16816<M>(sc[nt], a, qf[nt][ks][0], qf[nt][ks][1]);
         }
-        // a page's scales start on 128 bytes
-        const int kk = k_warp + g, sh = min(p.page_shift, 6), in_page = (1 << sh) - 1, pitch = max(32, 1 << sh);
         const float* scales = reinterpret_cast<const float*>(smem + s * C::STAGE + 2 * C::TILE);
-        const int at = (kk >> sh) * pitch + (kk & in_page);  // pages hold multiples of 16 keys: key g + 8 is in the same one
+        const int at = k_warp + g;
         const float ks0 = scales[at], ks1 = scales[at + 8];
         vs[0] = scales[C::SCALES / 4 + at];
         vs[1] = scales[C::SCALES / 4 + at + 8];

@@ -50,6 +50,7 @@ template <> struct Half8<__half> {
       f[2 * i + 1] = t.y;
     }
   }
+  __device__ static __forceinline__ float2 pair(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
   __device__ static __forceinline__ uint4 from_float(const float (&f)[8]) {
     uint4 u;
     __half2* h = reinterpret_cast<__half2*>(&u);
@@ -74,6 +75,9 @@ template <> struct Half8<__nv_bfloat16> {
       f[2 * i] = t.x;
       f[2 * i + 1] = t.y;
     }
+  }
+  __device__ static __forceinline__ float2 pair(uint32_t u) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&u));
   }
   __device__ static __forceinline__ uint4 from_float(const float (&f)[8]) {
     uint4 u;
