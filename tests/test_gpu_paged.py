@@ -4,6 +4,7 @@ import pytest
 import torch
 
 import tribench_b200 as tb
+import tribench_b200._native  # noqa: F401
 from paged_ref import attend, held, make_case
 
 pytestmark = pytest.mark.gpu
@@ -97,6 +98,22 @@ def test_ties_round_to_even():
     assert float(cache.k_scale[0, 0, 0]) == 1.0
 
 
+@pytest.mark.parametrize("top", [1e-39, 1e-35, 2.0 ** -100, 1e-20, 1e20, 1e33, 3.3e38])
+def test_rows_of_any_size(top):
+    """Codes of bf16 rows at both ends of the type's range, subnormal ones among them: the nearest, as 64 bits say."""
+    cache = tb.PagedKVCache.empty(1, 16, 1, 128, BF16, DEV, storage="int8")
+    x = (torch.rand(16, 1, 128, device=DEV, dtype=torch.float64) * 2 - 1).mul_(top).to(BF16)
+    table = torch.zeros(1, 1, dtype=torch.int32, device=DEV)
+    lens, cu = torch.tensor([16], dtype=torch.int32, device=DEV), torch.tensor([0, 16], dtype=torch.int32, device=DEV)
+    cache.append(x, x, table, lens, cu)
+    y = x.double()[:, 0]
+    a = y.abs().amax(-1, keepdim=True)
+    want = torch.round(y * 127 / a)
+    assert torch.equal(cache.k[0, 0].double(), want) and torch.equal(cache.v[0, 0].double(), want)
+    # a subnormal scale keeps fewer bits: half of the least subnormal, 2^-149
+    assert bool(((cache.k_scale[0, 0].double() - a[:, 0] / 127).abs() <= a[:, 0] / 127 * 2.0 ** -24 + 2.0 ** -150).all())
+
+
 def test_rows_that_are_not_finite_read_back_as_nan():
     cache = tb.PagedKVCache.empty(1, 16, 1, 64, BF16, DEV, storage="int8")
     x = torch.ones(3, 1, 64, device=DEV, dtype=BF16)
@@ -165,6 +182,10 @@ CASES = [
     ([300, 40], [20, 3000], 7, 1, 128, 16, BF16, "16bit", {}),
     ([130], [130], 128, 1, 64, 16, F16, "16bit", {}),
     ([40], [200], 160, 1, 64, 16, BF16, "int8", {}),
+    ([3, 2], [1000, 64], 20, 2, 128, 16, F16, "int8", {}),
+    ([4, 1], [63, 700], 8, 1, 64, 64, BF16, "int8", {"layout": "NHD", "mean": True}),
+    ([9], [2000], 24, 8, 128, 1024, F16, "16bit", {}),
+    ([50], [3000], 200, 1, 128, 32, F16, "16bit", {}),
 ]
 MASKS = [dict(), dict(window=1), dict(window=50, sinks=4), dict(window=200, sinks=70), dict(window=64), dict(causal=False)]
 
@@ -226,6 +247,101 @@ def test_strided_queries_and_outputs_and_rows_behind_the_last_sequence(max_new):
     tb.run_paged_attn(q, cache_of(c), c["table"], c["lens"], c["cu"], max_seqlen_q=max_new, out=q, sm_scale=0.3)  # in place
     n = sum(new)
     assert torch.equal(q[:n], o[:n])
+
+
+@pytest.mark.parametrize("n,hq", [(1, 2), (3, 16), (2, 8)])
+@pytest.mark.parametrize("storage", ["16bit", "int8"])
+def test_many_sequences(n, hq, storage):
+    """More sequences than threads of a block, and more blocks of query rows than the schedule keeps at hand."""
+    B = 2100
+    c = make_case(DEV, new=[1 + i % n for i in range(B)], past=[i * 7 % 40 for i in range(B)], hq=hq, hkv=2, dim=64, page=16,
+                  dtype=F16, storage=storage, seed=14)
+    o = tb.run_paged_attn(c["q"], cache_of(c), c["table"], c["lens"], c["cu"], max_seqlen_q=n)
+    check(c, o)
+    # a larger bound on the new tokens, and so another kernel, changes roundings only
+    o = tb.run_paged_attn(c["q"], cache_of(c), c["table"], c["lens"], c["cu"])
+    check(c, o)
+
+
+@pytest.mark.parametrize("n", [4, 100])
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_hidden_keys_and_values_weigh_nothing(n, dtype):
+    """The last token's key and value are the largest of the type: tokens before it do not notice."""
+    c = make_case(DEV, new=[n], past=[150], hq=4, hkv=2, dim=128, page=16, dtype=dtype, seed=15)
+    big = torch.finfo(dtype).max
+    last = 150 + n - 1
+    pg, row = int(c["table"][0, last // 16]), last % 16
+    c["v"][pg, :, row] = big
+    c["k"][pg, :, row] = torch.where(torch.rand(2, 128, device=DEV) < 0.5, -big, big).to(dtype)
+    o = tb.run_paged_attn(c["q"], cache_of(c), c["table"], c["lens"], c["cu"], max_seqlen_q=n)
+    want, bound = attend(c)
+    assert bool(((o[:n - 1].double() - want[:n - 1]).abs() <= bound[:n - 1]).all())
+
+
+@pytest.mark.parametrize("n", [1, 5, 100])
+def test_unused_scales_may_hold_anything(n):
+    for fill in (1e30, float("inf"), -5.0, 0.0):
+        c = make_case(DEV, new=[n, n], past=[70, 5], hq=4, hkv=2, dim=64, page=32, dtype=F16, storage="int8", seed=16)
+        for x in ("k_scale", "v_scale"):
+            c["kw"][x].nan_to_num_(nan=fill)
+        for mask in (dict(), dict(window=20, sinks=2)):
+            o = tb.run_paged_attn(c["q"], cache_of(c), c["table"], c["lens"], c["cu"], max_seqlen_q=n, **mask)
+            check(c, o, **mask)
+
+
+def test_values_of_very_different_sizes_in_an_int8_cache():
+    """The unit of the weights follows the largest scale seen; what came before it is rescaled."""
+    for n in (1, 100):
+        c = make_case(DEV, new=[n], past=[900], hq=4, hkv=2, dim=128, page=16, dtype=BF16, storage="int8", seed=17)
+        s = c["kw"]["v_scale"]
+        for j in range(0, 900 + n, 16):
+            s[c["table"][0, j // 16].long()] *= 2.0 ** (j / 40 - 10)
+        o = tb.run_paged_attn(c["q"], cache_of(c), c["table"], c["lens"], c["cu"], max_seqlen_q=n)
+        check(c, o)
+
+
+def test_a_slice_of_a_wider_page_table():
+    c = make_case(DEV, new=[1, 40, 3], past=[100, 30, 0], hq=4, hkv=2, dim=64, page=16, dtype=F16, seed=18)
+    wide = torch.full((3, 40), -1, dtype=torch.int32, device=DEV)
+    w = c["table"].shape[1]
+    wide[:, 7:7 + w] = c["table"]
+    a, b = (tb.run_paged_attn(c["q"], cache_of(c), t, c["lens"], c["cu"], max_seqlen_q=40) for t in (c["table"], wide[:, 7:7 + w]))
+    assert torch.equal(a, b)
+    check(c, a)
+
+
+def test_refusals_of_the_python_layer():
+    c = make_case(DEV, new=[1, 2], past=[3, 0], hq=4, hkv=2, dim=64, page=16, dtype=F16, seed=19)
+    cache = cache_of(c)
+    q, table, lens, cu = c["q"], c["table"], c["lens"], c["cu"]
+    kv = torch.zeros(3, 2, 64, dtype=F16, device=DEV)
+
+    def attn(q=q, table=table, lens=lens, cu=cu, **kw):
+        return tb.run_paged_attn(q, cache, table, lens, cu, **kw)
+
+    for err, text, call in (
+            (TypeError, "int32", lambda: attn(lens=lens.long())), (ValueError, "CUDA", lambda: attn(table=table.cpu())),
+            (ValueError, "dimension", lambda: attn(table=table[0])), (ValueError, "batch", lambda: attn(lens=lens[:1])),
+            (ValueError, "batch", lambda: attn(cu=cu[:2])), (ValueError, "columns", lambda: attn(table=table[:, :0])),
+            (ValueError, "stride 1", lambda: attn(table=table.t().contiguous().t())),
+            (TypeError, "dtype", lambda: attn(q=q.bfloat16())), (ValueError, "packed", lambda: attn(q=q[0])),
+            (ValueError, "differs", lambda: attn(out=torch.zeros(5, 4, 64, dtype=F16, device=DEV))),
+            (ValueError, "stride 1", lambda: attn(q=q.transpose(1, 2).contiguous().transpose(1, 2))),
+            (ValueError, "window", lambda: attn(window=0)), (tb._native.SageError, "causal", lambda: attn(window=4, causal=False)),
+            (tb._native.SageError, "window", lambda: attn(sinks=4)), (tb._native.SageError, "multiple", lambda: attn(q=q[:, :3])),
+            (tb._native.SageError, "one token", lambda: attn(cu=None)), (tb._native.SageError, "overlaps k", lambda: attn(out=c["k"][:3, 0, :4])),
+            (ValueError, "total", lambda: cache.gather(table, lens, cu)), (ValueError, "tokens", lambda: cache.append(kv, kv[:2], table, lens, cu)),
+            (TypeError, "dtype", lambda: cache.append(kv.float(), kv, table, lens, cu)),
+            (tb._native.SageError, "overlap", lambda: cache.gather(table, lens, cu, out=(kv, kv))),
+            (ValueError, "one shape", lambda: tb.PagedKVCache(c["k"], c["v"][:1])),
+            (TypeError, "int8", lambda: tb.PagedKVCache(c["k"].to(torch.int8), c["v"].to(torch.int8))),
+            (ValueError, "belong", lambda: tb.PagedKVCache(c["k"], c["v"], k_mean=kv[0].float())),
+            (tb._native.SageError, "page_size", lambda: tb.PagedKVCache.empty(4, 24, 2, 64, F16, DEV).append(kv, kv, table, lens, cu)),
+            (tb._native.SageError, "head_dim", lambda: tb.PagedKVCache.empty(4, 16, 2, 32, F16, DEV).append(kv[..., :32], kv[..., :32], table, lens, cu)),
+    ):
+        with pytest.raises(err, match=text):
+            call()
+    assert tb.device_status(DEV) == 0
 
 
 @pytest.mark.parametrize("storage", ["16bit", "int8"])

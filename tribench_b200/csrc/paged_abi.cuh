@@ -179,9 +179,14 @@ ChunkTile chunk_tile(int64_t G) {
 // Blocks of query rows of a call: a sequence's last block may be partly filled.
 int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q / (2 * chunk_tile(G).TT) + batch; }
 
-// Which kernel: an item of 16 query rows per key/value head streams the cache once per item, so a
-// sequence of more rows reads it several times; from there on the tensor-core tiles of 256 rows win.
-bool chunk_route(int64_t max_seqlen_q, int64_t G) { return max_seqlen_q * G > sage::kDecMaxRows; }
+// Which kernel. sage_decode.cuh streams the cache once per 16 query rows of a key/value head, at HBM's
+// rate; sage_chunk.cuh once per 256, at a rate that the softmax of a 128-row tile sets. Above 16 rows the
+// second wins over a 16-bit cache (32 rows over 16 sequences of 20000: 239 instead of 392 us), above 32
+// over an INT8 one, whose codes cost it more (17 to 32 rows: 341 instead of 309 us; 64: 343 instead of
+// 592). The largest sequence's rows decide, so that a mixed batch takes one kernel.
+bool chunk_route(int64_t max_seqlen_q, int64_t G, const sage_paged_cache* c) {
+  return max_seqlen_q * G > (c->storage == SAGE_CACHE_INT8 ? 2 : 1) * sage::kDecMaxRows;
+}
 
 // Tensor map of the packed queries: boxes of Gp heads by TT tokens by 64 channels.
 int query_map(CUtensorMap* map, const void* q, int dtype, int64_t D, int64_t heads, int64_t tokens, int64_t sh, int64_t st,
@@ -289,7 +294,7 @@ size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q
   if (!cache || heads_q <= 0 || batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || pages_per_seq <= 0) return 0;
   if (cache->heads_kv <= 0 || heads_q % cache->heads_kv) return 0;
   const int64_t G = heads_q / cache->heads_kv;
-  if (chunk_route(max_seqlen_q, G))
+  if (chunk_route(max_seqlen_q, G, cache))
     return chunk_ws(cache->head_dim, chunk_items(batch, total_q, G)).bytes;
   return decode_ws_bytes(cache->head_dim);
 }
@@ -348,7 +353,7 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* w = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(w);
-  const bool chunk = chunk_route(max_seqlen_q, G);
+  const bool chunk = chunk_route(max_seqlen_q, G, c);
   const int tile = chunk ? 128 : sage::kDecKeys;  // keys of a tile
   PagedMaps m;
   // the chunk kernel widens INT8 codes itself, from rows as they are

@@ -6,11 +6,13 @@
 // keeps the values. INT8 storage keeps, per (token, head) row x of D values (K: x - mean of its
 // head and channel, where the cache has a mean):
 //   a = max |x|, scale = a / 127, code = rint(127 x / a) (ties to even; a = 0: code 0)
-// and reads back code * scale (+ mean), rounded once to 16 bits. 127 x is exact in fp32 for 16-bit
-// x, and one correctly rounded division follows, so the code is the mathematically nearest one:
-// a quotient of integers of <= 18 and <= 11 bits that is no tie is >= 2^-12 away from one, far more
-// than half an ulp of a value below 128 (2^-18). A row that holds an infinity or a NaN gets
-// a = inf / NaN as its maximum and reads back as NaN.
+// and reads back code * scale (+ mean), rounded once to 16 bits. For 16-bit x without a mean 127 x is
+// exact in fp32 and one correctly rounded division follows, so the code is the mathematically nearest
+// one: with significands X, A < 2^11 and x = 2^-k X, a = A (k >= 0), 127 x / a misses a tie that it is
+// not on by at least 1 / (2 A 2^k) > 2^-12-k, while it is below 2^8-k and so rounded by less than
+// 2^-16-k. A row that holds an infinity or a NaN gets a = inf / NaN as its maximum and reads back as NaN.
+// Two new tokens of a call that name the same place leave either's values, of an INT8 cache possibly
+// one's codes under the other's scale.
 //
 // Both kernels move each byte once (write: 2 D in, 2 D or D + 4 out per row; read the inverse):
 // HBM bounds them for prompts, launch latency for single tokens.
@@ -88,25 +90,26 @@ __device__ __forceinline__ int find_seq(const int* cu, int batch, int row) {
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 
 // Eight INT8 codes rint(127 f / a) of f, |f| <= a, with the largest |f| of the row a.
-__device__ __forceinline__ uint2 codes_of(const float (&f)[8], float a) {
+__device__ __forceinline__ uint2 codes_of(float (&f)[8], float a) {
+  if (!(a > 7.9e-31f && a < 1.2e30f)) {  // beyond 2^-100 .. 2^100 (rare): brought inside by a power of two
+    if (!(a > 0.0f && a < INFINITY)) return make_uint2(0u, 0u);
+    const float s = a < 1.0f ? 18446744073709551616.0f : 5.421010862427522e-20f;  // 2^64, 2^-64
+    a *= s;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] *= s;
+  }
+  // The correctly rounded quotient (quotient_rn), two lanes at a time; adding 1.5 * 2^23 rounds it to an
+  // integer, ties to even, whose two's complement byte is the sum's lowest.
+  const float r = __frcp_rn(a);
+  const float2 r2 = make_float2(r, r), na2 = make_float2(-a, -a);
   uint32_t c[8];
-  if (a > 7.9e-31f && a < 1.2e30f) {  // 2^-100 .. 2^100: nothing below over- or underflows
-    // The correctly rounded quotient (quotient_rn), two lanes at a time; adding 1.5 * 2^23 rounds it to
-    // an integer, ties to even, whose two's complement byte is the sum's lowest.
-    const float r = __frcp_rn(a);
-    const float2 r2 = make_float2(r, r), na2 = make_float2(-a, -a);
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float2 x = fmul2(make_float2(f[e], f[e + 1]), make_float2(127.0f, 127.0f));
-      const float2 q = fmul2(x, r2);
-      const float2 z = fadd2(ffma2(ffma2(na2, q, x), r2, q), make_float2(12582912.0f, 12582912.0f));
-      c[e] = __float_as_uint(z.x);
-      c[e + 1] = __float_as_uint(z.y);
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)  // NaN (0 / 0, inf / inf) converts to 0
-      c[e] = (uint32_t)min(max(__float2int_rn(__fdiv_rn(__fmul_rn(f[e], 127.0f), a)), -127), 127);
+  for (int e = 0; e < 8; e += 2) {
+    const float2 x = fmul2(make_float2(f[e], f[e + 1]), make_float2(127.0f, 127.0f));
+    const float2 q = fmul2(x, r2);
+    const float2 z = fadd2(ffma2(ffma2(na2, q, x), r2, q), make_float2(12582912.0f, 12582912.0f));
+    c[e] = __float_as_uint(z.x);
+    c[e + 1] = __float_as_uint(z.y);
   }
   return make_uint2(pack4_lo_bytes(c[0], c[1], c[2], c[3]), pack4_lo_bytes(c[4], c[5], c[6], c[7]));
 }
