@@ -363,7 +363,8 @@ typedef struct sage_paged_cache {
 /*
  * Write new tokens' keys and values (packed [tokens, heads_kv, head_dim], element strides
  * {head, token}) into the cache. SAGE_CACHE_INT8 stores, per row x (K: x - k_mean) of head_dim
- * values, scale = max|x| / 127 and codes rint(127 x / max|x|), ties to even.
+ * values, scale = max|x| / 127 and codes rint(127 x / max|x|), ties to even. No two new tokens of a
+ * call may name the same place: the result is then either's, possibly one's codes under the other's scale.
  */
 int sage_paged_append(const sage_paged_cache* cache, const void* k, const void* v, const int64_t k_strides[2],
                       const int64_t v_strides[2], const int32_t* page_table, int64_t table_stride,

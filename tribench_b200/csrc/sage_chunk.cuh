@@ -30,6 +30,10 @@
 // MUFU.ex2: the polynomial share that sage_attn.cuh computes on the FMA pipe costs more here (12 of 32
 // columns: 16 bit 243 -> 231 us, INT8 540 -> 475 us without).
 //
+// Measured (B200, two chunks of 1024 tokens over 7168, 32/8 heads, head_dim 128): bf16 227 us, 1136
+// TFLOP/s; INT8 (fp16) 341 us; head_dim 64: 194 us (663 TFLOP/s) and 308 us. A tile of 128 keys takes
+// about 4100 clk, the chain S -> softmax -> P V -> next S of the two query tiles in turn.
+//
 // Warps: 0-7 softmax (two warpgroups), 8 TMA producer of K and V, 9 MMA issuer, 10 loads the next
 // segment's queries as soon as the last Q K^T of this one has run, 11 puts zeros over rows of V that no
 // query sees (an unused row may hold a NaN, which its weight of 0 would not silence). INT8: 8 loads

@@ -33,6 +33,9 @@
 // seen (raised when one exceeds it by 2^5). bf16 queries are brought to fp16 by a power of two per
 // row: 8 significant bits fit into 11, and what falls below 2^-24 of the row's largest value is lost
 // far under bf16's own rounding.
+//
+// Measured (B200, one token of each of 16 sequences of 20000, 64/8 heads, head_dim 128): 16 bit 200 us,
+// 6.55 TB/s, the rate of a plain copy; INT8 117 us, 5.6 TB/s of codes (issue slots 53 % busy).
 #pragma once
 
 #include <type_traits>
@@ -87,7 +90,8 @@ struct DecodeCfg {
   static constexpr int OFF_ML = OFF_RED + kDecWarps * ROWS * RED_STRIDE * 4;
   static constexpr int OFF_BAR = OFF_ML + kDecWarps * ROWS * 4 * 4;
   static constexpr int OFF_MISC = OFF_BAR + 2 * NS * 8;
-  static constexpr int SMEM = 1024 + OFF_MISC + 64;
+  static constexpr int OFF_SEG = (OFF_MISC + 56 + 15) / 16 * 16;
+  static constexpr int SMEM = 1024 + OFF_SEG + 64;
   static_assert(CTAS * (SMEM + 1024) <= 228 * 1024, "CTAs per SM");
 };
 
@@ -108,6 +112,14 @@ __device__ __forceinline__ TileSpan tile_span(const PagedSeq& q, int window, int
   return t;
 }
 __device__ __forceinline__ int tile_at(const TileSpan& t, int i) { return i < t.ns ? i : t.tw + i - t.ns; }
+
+// One segment of a CTA's piece: tiles [t0, t0 + n) of an item.
+struct DecodeSegment {
+  PagedSeq sq;
+  TileSpan ts;
+  int b, h, mt, t0, n, more;
+};
+static_assert(sizeof(DecodeSegment) <= 64, "DecodeCfg::SMEM");
 
 template <int ROWS>
 __device__ __forceinline__ int64_t decode_tiles(const DecodeParams& p, int b) {
@@ -323,15 +335,30 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
   int it = 0;
   bool ok = true;
   int4 cut = make_int4(0, 0, 0, 0);  // the item that this piece begins and does not end
-  while (left > 0 && b < p.s.batch) {
-    const PagedSeq sq = paged_seq(p.s, b);
-    const TileSpan ts = tile_span(sq, p.window, p.sinks, kDecKeys);
-    const int nmt = (sq.n * p.G + C::ROWS - 1) / C::ROWS;
-    const int64_t all = (int64_t)p.Hkv * nmt * ts.count;
-    if (rem >= all) { rem = 0; ++b; continue; }
-    const int item = (int)(rem / ts.count), t0 = (int)(rem - (int64_t)item * ts.count);
-    const int h = item / nmt, mt = item - h * nmt;
-    const int n = (int)min((int64_t)(ts.count - t0), left);
+  DecodeSegment& seg = *reinterpret_cast<DecodeSegment*>(smem + C::OFF_SEG);
+  for (;;) {
+    // One thread finds the segment for all: the warps meet at barriers, so they must agree on it even
+    // if the arrays change under a running call.
+    if (threadIdx.x == 0) {
+      seg.more = 0;
+      for (; left > 0 && b < p.s.batch; ++b, rem = 0) {
+        const PagedSeq sq = paged_seq(p.s, b);
+        const TileSpan ts = tile_span(sq, p.window, p.sinks, kDecKeys);
+        const int nmt = (sq.n * p.G + C::ROWS - 1) / C::ROWS;
+        if (rem >= (int64_t)p.Hkv * nmt * ts.count) continue;
+        const int item = (int)(rem / ts.count), t0 = (int)(rem - (int64_t)item * ts.count), h = item / nmt;
+        const int n = (int)min((int64_t)(ts.count - t0), left);
+        seg = DecodeSegment{sq, ts, b, h, item - h * nmt, t0, n, 1};
+        rem += n;
+        left -= n;
+        break;
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(kDecWarps * 32) : "memory");
+    if (!seg.more) break;
+    const PagedSeq sq = seg.sq;
+    const TileSpan ts = seg.ts;
+    const int h = seg.h, mt = seg.mt, t0 = seg.t0, n = seg.n;
     const int rows = min(C::ROWS, sq.n * p.G - mt * C::ROWS);  // valid rows of the item
     const int first = sq.len - sq.n;                           // position of the first new token
     // This thread's query rows 8 nt + 2 t, 8 nt + 2 t + 1: the keys [lo, hi) (and [0, sinks)) that they see
@@ -703,10 +730,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
         if (c4 == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * C::ROWS + row) * 4) = make_float4(ms, sum, mo, 0.0f);
       }
     }
-    if (begins && !ends) cut = make_int4(b, h, mt, (int)((ts.count - n + per - 1) / per));
+    if (begins && !ends) cut = make_int4(seg.b, h, mt, (int)((ts.count - n + per - 1) / per));
     asm volatile("bar.sync 1, %0;" ::"n"(kDecWarps * 32) : "memory");
-    rem += n;
-    left -= n;
   }
   if (threadIdx.x == 0) p.desc[cta] = cut;
 }

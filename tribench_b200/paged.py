@@ -179,7 +179,9 @@ class PagedKVCache:
         return cls(k, v, **scales, k_mean=k_mean, dtype=dtype, tensor_layout=tensor_layout)
 
     def append(self, k, v, page_table, seq_lens, cu_seqlens=None):
-        """Write the new tokens' keys and values ([tokens, heads_kv, head_dim] in the cache's dtype)."""
+        """Write the new tokens' keys and values ([tokens, heads_kv, head_dim] in the cache's dtype).
+
+        No two new tokens of a call may name the same place (two sequences that write into a shared page)."""
         tokens, ks = _packed2("k", k, self.heads_kv, self.head_dim, self.dtype, self.device)
         tv, vs = _packed2("v", v, self.heads_kv, self.head_dim, self.dtype, self.device)
         if tv != tokens:
