@@ -186,6 +186,11 @@ CASES = [
     ([4, 1], [63, 700], 8, 1, 64, 64, BF16, "int8", {"layout": "NHD", "mean": True}),
     ([9], [2000], 24, 8, 128, 1024, F16, "16bit", {}),
     ([50], [3000], 200, 1, 128, 32, F16, "16bit", {}),
+    # single tokens beside chunks: two kernels, each on its sequences
+    ([1] * 19 + [200], [(i * 377) % 900 for i in range(20)], 8, 2, 128, 16, BF16, "16bit", {}),
+    ([2, 1, 0, 1, 90, 1, 5, 4] + [1] * 10, [30, 0, 4, 700, 64, 63, 12, 1000] + [9] * 10, 8, 2, 64, 32, F16, "16bit", {}),
+    ([1, 300, 2, 1, 1, 8, 0] + [1] * 30, [100, 0, 65, 3000, 1, 20, 3] + [77] * 30, 12, 2, 128, 64, BF16, "int8", {"mean": True}),
+    ([1, 1, 40, 1, 1] + [1] * 20, [10, 20, 200, 640, 0] + [130] * 20, 20, 1, 64, 16, F16, "int8", {}),
 ]
 MASKS = [dict(), dict(window=1), dict(window=50, sinks=4), dict(window=200, sinks=70), dict(window=64), dict(causal=False)]
 

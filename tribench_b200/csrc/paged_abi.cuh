@@ -183,9 +183,20 @@ int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q 
 // rate; sage_chunk.cuh once per 256, at a rate that the softmax of a 128-row tile sets. Above 16 rows the
 // second wins over a 16-bit cache (32 rows over 16 sequences of 20000: 239 instead of 392 us), above 32
 // over an INT8 one, whose codes cost it more (17 to 32 rows: 341 instead of 309 us; 64: 343 instead of
-// 592). The largest sequence's rows decide, so that a mixed batch takes one kernel.
-bool chunk_route(int64_t max_seqlen_q, int64_t G, const sage_paged_cache* c) {
-  return max_seqlen_q * G > (c->storage == SAGE_CACHE_INT8 ? 2 : 1) * sage::kDecMaxRows;
+// 592).
+int64_t few_rows(const sage_paged_cache* c) { return (c->storage == SAGE_CACHE_INT8 ? 2 : 1) * sage::kDecMaxRows; }
+// Sequences from which two kernels pay: 64 single tokens over up to 8192 beside a chunk of 512, 32/8 heads: 311
+// instead of 377 us (INT8 237 instead of 628); 8 sequences 39 instead of 31 us, the price of two more launches.
+constexpr int64_t kMixedBatch = 16;
+enum class PagedRoute { kFew, kMany, kBoth };
+// Of a batch the host knows the largest sequence's rows and the others' mean. Where the largest has many
+// and the others have few on average (single tokens beside a chunk), both kernels run, each on the
+// sequences of its kind; else the largest decides.
+PagedRoute paged_route(const sage_paged_cache* c, int64_t G, int64_t batch, int64_t total_q, int64_t max_seqlen_q) {
+  const int64_t few = few_rows(c);
+  if (max_seqlen_q * G <= few) return PagedRoute::kFew;
+  const bool mixed = batch >= kMixedBatch && (total_q - std::min(max_seqlen_q, total_q)) * G <= few * (batch - 1);
+  return mixed ? PagedRoute::kBoth : PagedRoute::kMany;
 }
 
 // Tensor map of the packed queries: boxes of Gp heads by TT tokens by 64 channels.
@@ -294,9 +305,10 @@ size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q
   if (!cache || heads_q <= 0 || batch <= 0 || total_q <= 0 || max_seqlen_q <= 0 || pages_per_seq <= 0) return 0;
   if (cache->heads_kv <= 0 || heads_q % cache->heads_kv) return 0;
   const int64_t G = heads_q / cache->heads_kv;
-  if (chunk_route(max_seqlen_q, G, cache))
-    return chunk_ws(cache->head_dim, chunk_items(batch, total_q, G)).bytes;
-  return decode_ws_bytes(cache->head_dim);
+  // the two kernels of a mixed batch run one after the other in the same workspace
+  const PagedRoute route = paged_route(cache, G, batch, total_q, max_seqlen_q);
+  const size_t many = route == PagedRoute::kFew ? 0 : chunk_ws(cache->head_dim, chunk_items(batch, total_q, G)).bytes;
+  return std::max(many, route == PagedRoute::kMany ? size_t(0) : decode_ws_bytes(cache->head_dim));
 }
 
 int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int64_t q_strides[2], void* o,
@@ -353,21 +365,36 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   char* w = static_cast<char*>(workspace);
   p.part = reinterpret_cast<float*>(w);
-  const bool chunk = chunk_route(max_seqlen_q, G, c);
-  const int tile = chunk ? 128 : sage::kDecKeys;  // keys of a tile
-  PagedMaps m;
-  // the chunk kernel widens INT8 codes itself, from rows as they are
-  if (int rc = cache_map(&m.k, c, false, tile, !chunk)) return rc;
-  if (int rc = cache_map(&m.v, c, true, tile, !chunk)) return rc;
-  if (chunk) {
-    sage::ChunkParams cp{};
+  const PagedRoute route = paged_route(c, G, batch, total_q, max_seqlen_q);
+  p.s.group = (int)G;
+  if (route != PagedRoute::kMany) {
+    if (route == PagedRoute::kBoth) { p.s.rows_lo = 1; p.s.rows_hi = (int)few_rows(c); }
+    PagedMaps m;
+    if (int rc = cache_map(&m.k, c, false, sage::kDecKeys)) return rc;
+    if (int rc = cache_map(&m.v, c, true, sage::kDecKeys)) return rc;
+    const size_t rows = size_t(2) * sage::kDecMaxPieces * sage::kDecMaxRows;
+    p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
+    p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
+    // rows of an item, at most: of a mixed batch 8 where a single token's fit (a few tokens' take several items)
+    const int max_rows = route == PagedRoute::kBoth ? (G <= 8 ? 8 : sage::kDecMaxRows)
+                                                    : (int)std::min<int64_t>(G * p.s.max_new, sage::kDecMaxRows);
+    if (int rc = D == 128 ? decode_dispatch<128>(i8, bf, m, p, max_rows, st) : decode_dispatch<64>(i8, bf, m, p, max_rows, st))
+      return rc;
+  }
+  if (route != PagedRoute::kFew) {
+    if (route == PagedRoute::kBoth) { p.s.rows_lo = (int)few_rows(c) + 1; p.s.rows_hi = 0x7fffffff; }
+    const ChunkTile t = chunk_tile(G);
+    PagedMaps m;
+    // the kernel widens INT8 codes itself, from rows as they are
+    if (int rc = cache_map(&m.k, c, false, 128, false)) return rc;
+    if (int rc = cache_map(&m.v, c, true, 128, false)) return rc;
+    if (int rc = query_map(&m.q, q, c->dtype, D, heads_q, total_q, q_strides[0], q_strides[1], t)) return rc;
     const int64_t items = chunk_items(batch, total_q, G);
     const ChunkWs o = chunk_ws(D, items);
-    const ChunkTile t = chunk_tile(G);
-    if (int rc = query_map(&m.q, q, c->dtype, D, heads_q, total_q, q_strides[0], q_strides[1], t)) return rc;
-    p.parts = (int)t.parts; p.Gp = (int)t.Gp; p.TT = (int)t.TT;
     p.part_ml = reinterpret_cast<float*>(w + o.ml);
     p.desc = reinterpret_cast<int4*>(w + o.desc);
+    p.parts = (int)t.parts; p.Gp = (int)t.Gp; p.TT = (int)t.TT;
+    sage::ChunkParams cp{};
     cp.d = p;
     cp.items = reinterpret_cast<sage::ChunkItem*>(w + o.items);
     cp.prefix = reinterpret_cast<int64_t*>(w + o.prefix);
@@ -376,11 +403,7 @@ int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int6
     if (i8) cp.c = paged_store(c);
     return D == 128 ? chunk_dispatch<128>(i8, bf, m, cp, st) : chunk_dispatch<64>(i8, bf, m, cp, st);
   }
-  const int max_rows = (int)std::min<int64_t>(G * p.s.max_new, sage::kDecMaxRows);
-  const size_t rows = size_t(2) * sage::kDecMaxPieces * sage::kDecMaxRows;
-  p.part_ml = reinterpret_cast<float*>(w + align256(rows * D * 4));
-  p.desc = reinterpret_cast<int4*>(w + align256(rows * D * 4) + align256(rows * 4 * 4));
-  return D == 128 ? decode_dispatch<128>(i8, bf, m, p, max_rows, st) : decode_dispatch<64>(i8, bf, m, p, max_rows, st);
+  return SAGE_OK;
 }
 
 }  // extern "C"

@@ -38,6 +38,9 @@ struct PagedSeqs {
   int tokens;        // rows of the packed tensor
   int max_new;       // no sequence has more new tokens
   int cap;           // width * page size, clamped to 2^30: no length goes past it
+  // Sequences whose query rows per key/value head (new tokens * group) lie outside [rows_lo, rows_hi] are
+  // left to another launch: they appear to have no new tokens. rows_hi 0: none is.
+  int group, rows_lo, rows_hi;
 };
 
 struct PagedSeq {
@@ -55,6 +58,7 @@ __device__ __forceinline__ PagedSeq paged_seq(const PagedSeqs& s, int b) {
     r.n = sp.len;
   }
   r.len = min(max(len, 0), s.cap);
+  if (s.rows_hi != 0 && (r.n * s.group < s.rows_lo || r.n * s.group > s.rows_hi)) r.n = 0;
   return r;
 }
 
