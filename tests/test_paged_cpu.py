@@ -118,6 +118,23 @@ def test_workspace_and_overlaps_are_checked(ptr):
             assert rc not in (N.SAGE_OK, N.SAGE_ERR_INVALID_ARG, N.SAGE_ERR_WORKSPACE)
 
 
+def test_workspace_covers_every_kernel_of_a_call(ptr):
+    """Few rows: a size of its own; many: one that grows with the blocks of rows; a mixed batch: the larger of the two."""
+    c = cache(ptr, head_dim=128, k_strides=(4096, 2048, 128), v_strides=(4096, 2048, 128))
+
+    def size(hq, batch, total, max_q):
+        return N.load().sage_paged_workspace_bytes(ctypes.byref(c), hq, batch, total, max_q, 64)
+
+    few = size(8, 32, 32, 1)
+    assert few > 0 and few == size(8, 1000, 2000, 2) == size(16, 1, 2, 2)
+    many = size(8, 2, 1000, 600)
+    assert size(8, 2, 100000, 60000) > many
+    mixed = size(8, 64, 63 + 512, 512)
+    assert mixed >= few and mixed >= size(8, 2, 63 + 512, 512)
+    for bad in ((0, 1, 1, 1), (8, 0, 1, 1), (8, 1, 0, 1), (8, 1, 1, 0), (3, 1, 1, 1)):
+        assert size(*bad) == 0
+
+
 def test_empty_calls_do_nothing(ptr):
     assert attn(ptr, total=0) == N.SAGE_OK and attn(ptr, batch=0, total=0, cu=None, table=None, lens=None) == N.SAGE_OK
     assert move(ptr, tokens=0) == N.SAGE_OK and move(ptr, "sage_paged_gather", tokens=0) == N.SAGE_OK
