@@ -36,7 +36,10 @@ from .sage_attn import _DTYPES, _check_tensor
 # short: stride arrays and workspace sizes are looked up by value, the stream and the current device
 # are asked for directly.
 _strides2 = functools.lru_cache(maxsize=1024)(N.strides2)
-_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _raw_stream(index: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 _HERE = contextlib.nullcontext()
