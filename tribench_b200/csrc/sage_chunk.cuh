@@ -20,9 +20,15 @@
 //
 // INT8 cache: helper warps turn the codes into fp16 tiles (exact) in shared memory, in the layout the
 // TMA load would give, and the scales stay out of the products: scores are multiplied by k_scale per
-// column in fp32, P by v_scale before it is rounded to fp16, in units of a power of two 2^E that
-// follows the largest v_scale of the segment (E is raised, and O rescaled, once a tile exceeds it by
-// 2^4; P < 2^8 * 2^5 stays inside fp16). bf16 queries are brought to fp16 by a power of two per row.
+// column in fp32, P by v_scale before it is rounded to fp16, in units of a power of two 2^E. Two ways:
+// - The tile's visible scales (other than 0) span less than 2^7, as those of most models do: one E for
+//   the tile, 2^E <= v_scale < 2^(E + 7), kept from tile to tile while it fits, else moved and O rescaled.
+//   P < 2^8 * 2^7 stays inside fp16, and what it loses below 2^(E - 25) is at most 2^-25 of v_scale.
+// - They span more, or E would move by more than 2^30 within a segment: E per query row, 2^E <= the
+//   largest P v_scale that the row has met, from the products themselves, for this tile and the rest of
+//   the segment. A key weighs by what it contributes to the row, whatever scales other keys have. The
+//   softmax loop stays the same: E goes into the exponent, and out of the sum of the tile.
+// bf16 queries are brought to fp16 by a power of two per row.
 //
 // Code size counts: the softmax's and the converters' loops run side by side on the same instruction
 // cache, and unrolled whole (22 KB of converter) the INT8 kernel took 475 us where this one takes 343
@@ -111,6 +117,9 @@ struct ChunkCfg {
   static constexpr uint32_t IDESC_PV = make_idesc(kFmtD_F32, FMT, FMT, 0, 1, BM, D);
   static constexpr float LAZY = 8.0f;
 };
+// INT8, added to a tile's E where every row finds its own unit. E is then kRowRange below the largest scale so
+// far: the row's unit may be kRowRange + 1 above E and 2^kRowDepth below before an exponential leaves fp32.
+constexpr int kRowUnits = 1 << 20, kRowRange = 60, kRowDepth = 118;
 
 // ------------------------------------------------------------------ schedule
 __device__ __forceinline__ int chunk_blocks(const ChunkParams& p, const PagedSeq& sq) {
@@ -474,7 +483,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       bool ok = true;
       for (; w.more() && ok; step()) {
         const int n = w.n, kvh = w.head / p.parts;
-        int hi, lo, ids = 0, e = -200;
+        int hi, lo, ids = 0;
+        int e = -126, e_first = 0;                 // the scales' unit; that of the segment's first tile
+        bool has_unit = false, row_units = false;  // e is set; the rows have units of their own
+        int unit = -126;                           // what the tile's v_scales are divided by (log2)
         seen(&hi, &lo);
         for (int j = 0; j < n; ++j, ++it) {
           const int s = it % C::NS;
@@ -494,22 +506,36 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           ok = __all_sync(0xffffffffu, ok);
           if (!ok) break;
           if (isv) {  // V's slot is free, so are the scales'
-            float m = 0.0f;
+            unsigned top = 0, low = 255;  // exponent fields of the visible scales other than 0 (and subnormal ones)
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
               const int kx = key + x;
               if (!(kx < hi && (kx >= lo || kx < p.sinks))) k4[x] = v4[x] = 0.0f;
-              m = fmaxf(m, v4[x]);
+              const unsigned f = (__float_as_uint(v4[x]) >> 23) & 255u;
+              top = max(top, f);
+              low = min(low, f ? f : 255u);
             }
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const int et = min(max((int)(__float_as_uint(m) >> 23) - 127, -126), 120);
-            if (e == -200 || et > e + 4) e = et;
-            const float down = pow2(-e);
+            const bool fits = has_unit && !row_units && (int)low >= e + 127 && (int)top <= e + 133;
+            if (!__all_sync(0xffffffffu, fits)) {
+              top = __reduce_max_sync(0xffffffffu, top);
+              low = __reduce_min_sync(0xffffffffu, low);
+              const int t_hi = (int)top - 127, t_lo = (int)low - 127;
+              if (top == 255u || (top && t_hi - t_lo > 6)) {
+                row_units = true;
+              } else if (top && (!has_unit || t_lo < e || t_hi > e + 6)) {
+                e = min(max(t_lo - (6 - (t_hi - t_lo)) / 2, -126), 121);
+                if (!has_unit) e_first = e;
+                has_unit = true;
+                row_units |= e > e_first + 30 || e < e_first - 30;
+              }
+              if (!row_units) unit = e;
+              else if (top) unit = max(unit, t_hi - kRowRange);  // never below what a row's unit may follow
+            }
+            const float down = pow2(-unit);
             float4* sc = reinterpret_cast<float4*>(smem + C::OFF_SCALE + s * 1024);
             sc[lane] = make_float4(k4[0], k4[1], k4[2], k4[3]);
             sc[32 + lane] = make_float4(v4[0] * down, v4[1] * down, v4[2] * down, v4[3] * down);
-            if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = e;
+            if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = row_units ? unit + kRowUnits : unit;
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_sc + s);
           }
@@ -775,6 +801,55 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       for (int j = 0; j < n; ++j) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar_sfull + t, (ct + j) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
         tc_fence_after();
+        float shrink = 1.0f;  // INT8: O's factor where the unit moves
+        int unit_shift = 0;   // INT8: the exponentials are divided by 2^unit_shift
+        float lazy = C::LAZY;
+        uint32_t scales = 0;
+        const int up = hi - key0, down = lo - key0, sk = p.sinks - key0;
+        if constexpr (I8) {
+          const int s = (it_seg + j) % C::NS;
+          if (!__all_sync(0xffffffffu, mbar_wait(bar_sc + s, ((it_seg + j) / C::NS) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
+          scales = smem_u32(smem + C::OFF_SCALE) + s * 1024;
+          const int e_tile = *reinterpret_cast<const int*>(smem + C::OFF_EXP + 4 * s);
+          int e = e_tile;
+          if (e_tile >= kRowUnits / 2) {
+            // Rare, and kept out of the code below: the row's unit, from its largest product, in two passes
+            // over S (32 columns at a time, from TMEM): the maximum, then the products.
+            const int et = e_tile - kRowUnits;
+            float m = m_run, top = 0.0f;
+#pragma unroll 1
+            for (int c0 = 0; c0 < 256; c0 += 32) {
+              const int k0 = c0 & 127;
+              uint32_t sr[32];
+              tmem_ld32_sync(s_tmem + k0, sr);
+              const float use = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+              for (int c = 0; c < 32; c += 4) {
+                float2 ks[2], vs[2];
+                ld_shared_f4(scales + 4 * (k0 + c), ks);
+                ld_shared_f4(scales + 512 + 4 * (k0 + c), vs);
+                const float k4[4] = {ks[0].x, ks[0].y, ks[1].x, ks[1].y}, v4[4] = {vs[0].x, vs[0].y, vs[1].x, vs[1].y};
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                  const int at = k0 + c + x;
+                  if (at < up && (at >= down || at < sk)) {
+                    const float b = __uint_as_float(sr[c + x]) * k4[x] * scale;
+                    if (c0 < 128) m = fmaxf(m, b);
+                    else top = fmaxf(top, fabsf(ex2_approx(b - use) * v4[x]));
+                  }
+                }
+              }
+            }
+            // the weights of before have shrunk by 2^(m - m_run), so may their unit
+            const int before = m_run == -INFINITY ? -126 : e_run - (int)ceilf(fminf(m - m_run, 256.0f));
+            e = min(max(max(top > 0.0f ? exponent(top) + et : -126, before), max(et - kRowDepth, -126)), 121);
+            if (m_run == -INFINITY) e_run = e;
+            unit_shift = e - et;
+            lazy = 0.0f;
+          }
+          if (j > 0 && e != e_run) shrink = pow2(min(max(e_run - e, -126), 126));
+          e_run = e;
+        }
         float b[128];
         {
           uint32_t sr[128];
@@ -786,16 +861,8 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
 #pragma unroll
           for (int c = 0; c < 128; ++c) b[c] = __uint_as_float(sr[c]);
         }
-        float shrink = 1.0f;  // INT8: O's factor where the unit is raised
-        uint32_t scales = 0;
         if constexpr (I8) {
-          const int s = (it_seg + j) % C::NS;
-          if (!__all_sync(0xffffffffu, mbar_wait(bar_sc + s, ((it_seg + j) / C::NS) & 1, abort_flag, kDevTimeoutSoftmax, p.wait_limit_ns))) { ok = false; break; }
-          scales = smem_u32(smem + C::OFF_SCALE) + s * 1024;
-          const int e = *reinterpret_cast<const int*>(smem + C::OFF_EXP + 4 * s);
           float2 ks4[4][2];
-          if (j > 0 && e != e_run) shrink = pow2(max(e_run - e, -126));
-          e_run = e;
 #pragma unroll
           for (int c = 0; c < 128; c += 4) {
             if (c % 16 == 0) {
@@ -808,7 +875,6 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             b[c] = x.x; b[c + 1] = x.y; b[c + 2] = y.x; b[c + 3] = y.y;
           }
         }
-        const int up = hi - key0, down = lo - key0, sk = p.sinks - key0;
         const bool masked = key0 + 128 > all_hi || (key0 < all_lo && key0 + 128 > p.sinks);
         if (masked) {
           uint32_t vis[4];  // bit c % 32 of word c / 32: this row sees key c of the tile
@@ -831,13 +897,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           hm[h2] = fmax3(fmax3(a[0], a[1], a[2]), fmax3(a[3], a[4], a[5]), fmaxf(a[6], a[7]));
         }
         const float tmax = fmaxf(hm[0], hm[1]) * scale;
-        const bool upd = tmax > m_run + C::LAZY;
+        const bool upd = tmax > m_run + (I8 ? lazy : C::LAZY);
         const float m_new = upd ? tmax : m_run;
         const float alpha = upd ? ex2_approx(m_run - m_new) : 1.0f;
-        const bool rescale = j > 0 && __any_sync(0xffffffffu, upd || (I8 && shrink != 1.0f));
-        const float m_use = (m_new == -INFINITY) ? 0.0f : m_new;
-        const float2 scv = make_float2(scale, scale), ccv = make_float2(-m_use, -m_use);
+        float m_use = (m_new == -INFINITY) ? 0.0f : m_new;
+        const float2 scv = make_float2(scale, scale);
+        if constexpr (I8) m_use += (float)unit_shift;
+        const float2 ccv = make_float2(-m_use, -m_use);
         float2 acc[4] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+        const bool rescale = j > 0 && __any_sync(0xffffffffu, upd || (I8 && shrink != 1.0f));
 #pragma unroll
         for (int h2 = 0; h2 < 2; ++h2) {
           uint32_t pk[32];
@@ -878,7 +946,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
         tc_fence_before();
         mbar_arrive(bar_pfull + t);
         const float2 s01 = fadd2(fadd2(acc[0], acc[1]), fadd2(acc[2], acc[3]));
-        l_run = fmaf(l_run, alpha, s01.x + s01.y);
+        l_run = I8 ? fmaf(l_run, alpha, (s01.x + s01.y) * pow2(unit_shift)) : fmaf(l_run, alpha, s01.x + s01.y);
         m_run = m_new;
         key0 = j == jump ? jump_to : key0 + 128;
       }
@@ -942,7 +1010,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                               __uint_as_float(orow[4 * v + 2]), __uint_as_float(orow[4 * v + 3]));
           }
         }
-        if (valid) *reinterpret_cast<float4*>(p.part_ml + (slot * kChunkRows + row) * 4) = make_float4(m_run, l_run, I8 ? m_run + e_run : m_run, 0.0f);
+        if (valid) *reinterpret_cast<float4*>(p.part_ml + (slot * kChunkRows + row) * 4) = make_float4(m_run, l_run, (float)e_run, 0.0f);
       }
       tc_fence_before();
     }
@@ -966,7 +1034,7 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) paged_chunk_join_kernel(con
   const int tok = (2 * d.z + (row >> 7)) * p.TT + rt;
   if (rt >= p.TT || tok >= sq.n || part * p.Gp + hd >= p.G) return;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  float m = -INFINITY, l = 0.0f, mo = -INFINITY;  // mo: INT8, the outputs' own unit
+  float m = I8 ? kNoScore : -INFINITY, l = 0.0f, eo = -126.0f;  // INT8: the outputs are in units of 2^(m + eo)
 #pragma unroll 4
   for (int j = 0; j <= d.w; ++j) {
     const int64_t slot = j == 0 ? 2 * blockIdx.x + 1 : 2 * (blockIdx.x + j);
@@ -974,20 +1042,20 @@ __global__ void __launch_bounds__(kJoinRows * D / 4) paged_chunk_join_kernel(con
     const float4 v = reinterpret_cast<const float4*>(p.part)[(slot * (D / 4) + x) * kChunkRows + row];
     const float mn = fmaxf(m, ml.x), use = mn == -INFINITY ? 0.0f : mn;
     float a = ex2_approx(m - use), z = ex2_approx(ml.x - use);
-    m = mn;
     l = fmaf(l, a, ml.y * z);
     if constexpr (I8) {
-      const float on = fmaxf(mo, ml.z), uo = on == -INFINITY ? 0.0f : on;
-      a = ex2_approx(mo - uo);
-      z = ex2_approx(ml.z - uo);
-      mo = on;
+      const float en = fmaxf(unit_under(m, eo, mn), unit_under(ml.x, ml.z, mn));
+      a = ex2_approx((m - mn) + (eo - en));
+      z = ex2_approx((ml.x - mn) + (ml.z - en));
+      eo = en;
     }
+    m = mn;
     o.x = fmaf(o.x, a, v.x * z);
     o.y = fmaf(o.y, a, v.y * z);
     o.z = fmaf(o.z, a, v.z * z);
     o.w = fmaf(o.w, a, v.w * z);
   }
-  const float inv = l == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - m) / l : 1.0f / l);
+  const float inv = l == 0.0f ? 0.0f : (I8 ? pow2((int)eo) : 1.0f) / l;
   T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(kvh * p.G + part * p.Gp + hd) * p.o_sh + x * 4;
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
 }

@@ -29,8 +29,11 @@
 //
 // INT8. K: byte c + 128 zero-extended is the fp16 subnormal (c + 128) 2^-24, exact, without an
 // instruction beyond the byte permutation; the scores become 2^24 S' - 128 sum(q), then times k_scale.
-// V: codes as exact fp16 values; its weights are p_j v_scale_j 2^-E, E following the largest v_scale
-// seen (raised when one exceeds it by 2^5). bf16 queries are brought to fp16 by a power of two per
+// V: codes as exact fp16 values; their weights w_j = p_j v_scale_j are rounded to fp16 in units of 2^E,
+// E per query row: 2^E <= the largest w_j that the row has met < 2^(E + 14), so a weight is off by 2^-11
+// of itself or 2^-25 of the largest one, whatever the scales of keys that the row does not see or hardly
+// attends to. Row maxima of the scores (for the sum) and units (for the outputs) move together, when a
+// weight or an exponential outgrows its range. bf16 queries are brought to fp16 by a power of two per
 // row: 8 significant bits fit into 11, and what falls below 2^-24 of the row's largest value is lost
 // far under bf16's own rounding.
 //
@@ -63,7 +66,7 @@ struct DecodeParams {
   int causal, window, sinks;       // window 0: none
   float scale_log2;                // sm_scale * log2(e)
   float* part;                     // [2 * CTAs][rows][D] unnormalised outputs
-  float* part_ml;                  // [2 * CTAs][rows][4]: max of scores, sum, unit of the outputs (log2)
+  float* part_ml;                  // [2 * CTAs][rows][4]: max of scores, sum, INT8: E of the outputs' unit 2^(max + E)
   int4* desc;                      // [CTAs]: the item that a CTA's piece begins and does not end (sequence,
                                    // head, query tile or block, pieces that follow with its rest; 0: none)
   // Rows of the chunk kernel's blocks: parts of a head group (1 up to 128 heads), query heads of a
@@ -174,7 +177,14 @@ __device__ __forceinline__ uint32_t movmatrix(uint32_t x) {
   return y;
 }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }  // -126 <= e <= 127
+// exponent of |x|, clamped to what pow2 takes either way
 __device__ __forceinline__ int exponent(float x) { return min(max((int)((__float_as_uint(x) >> 23) & 255) - 127, -126), 120); }
+
+// INT8: outputs in units of 2^(m + e) (m: maximum of the scores, e: exponent of the weights' unit), seen from a
+// maximum ms >= m: the exponent that is sure not to make them larger by 2 or more.
+__device__ __forceinline__ float unit_under(float m, float e, float ms) { return fmaxf(e + ceilf(m - ms), -126.0f); }
+// No score yet: finite, so that differences of maxima are numbers.
+constexpr float kNoScore = -3.402823466e38f;
 
 // T: element type of q, o and a 16-bit cache. NR: query rows of an item / 8.
 template <int D, bool I8, typename T, int NR>
@@ -452,10 +462,16 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
     float m1[NR][2], l[NR][2];  // l: this lane's part
 #pragma unroll
     for (int nt = 0; nt < NR; ++nt) {
-      m1[nt][0] = m1[nt][1] = -INFINITY;
+      m1[nt][0] = m1[nt][1] = I8 ? kNoScore : -INFINITY;
       l[nt][0] = l[nt][1] = 0.0f;
     }
-    int unit_v = -126;  // INT8: weights are in units of 2^unit_v
+    int unit[NR][2];    // INT8: weights are in units of 2^unit, down = 2^-unit
+    float down[NR][2];
+#pragma unroll
+    for (int nt = 0; nt < NR; ++nt) {
+      unit[nt][0] = unit[nt][1] = -126;
+      down[nt][0] = down[nt][1] = pow2(126);
+    }
 
 #pragma unroll 1
     for (int i = t0; i < t0 + n; ++i, ++it) {
@@ -545,70 +561,111 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
           }
         } else {
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {  // nor may an unused scale raise the unit
+          for (int x = 0; x < 2; ++x) {  // nor may an unused scale
             const int key = key0 + k_warp + x * 8 + g;
             if (!(key < any_hi && (key >= any_lo || key < p.sinks))) vs[x] = 0.0f;
           }
         }
       }
-      // ---- the maximum (and INT8's unit), where a score outgrew it
-      float down = 1.0f;
-      if constexpr (I8) down = pow2(-unit_v);
-      bool grow = I8 && fmaxf(vs[0], vs[1]) * down > 32.0f;
-#pragma unroll
-      for (int nt = 0; nt < NR; ++nt)
-        grow |= fmaxf(sc[nt][0], sc[nt][2]) > m1[nt][0] + LAZY || fmaxf(sc[nt][1], sc[nt][3]) > m1[nt][1] + LAZY;
-      if (__any_sync(0xffffffffu, grow)) {
-        float shrink = 1.0f;
-        if constexpr (I8) {
-          float mv = fmaxf(fmaxf(vs[0], vs[1]), 0.0f);
-#pragma unroll
-          for (int o = 4; o < 32; o <<= 1) mv = fmaxf(mv, __shfl_xor_sync(0xffffffffu, mv, o));
-          const int e = max(unit_v, exponent(mv));
-          shrink = pow2(max(unit_v - e, -126));
-          unit_v = e;
-          down = pow2(-e);
-        }
+      uint32_t pf[NR][2];  // weights, as the B operand of O^T = V^T P^T
+      if constexpr (!I8) {
+        // ---- the maximum, where a score outgrew it
+        bool grow = false;
 #pragma unroll
         for (int nt = 0; nt < NR; ++nt)
+          grow |= fmaxf(sc[nt][0], sc[nt][2]) > m1[nt][0] + LAZY || fmaxf(sc[nt][1], sc[nt][3]) > m1[nt][1] + LAZY;
+        if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
+          for (int nt = 0; nt < NR; ++nt)
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float mn = fmaxf(m1[nt][c], mx);
-            const float alpha = mn == -INFINITY ? 1.0f : ex2_approx(m1[nt][c] - mn);
-            m1[nt][c] = mn;
-            l[nt][c] *= alpha;
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
 #pragma unroll
-            for (int x = 0; x < NT; ++x) {
-              acc[x][nt][c] *= alpha * shrink;
-              acc[x][nt][c + 2] *= alpha * shrink;
+              for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const float mn = fmaxf(m1[nt][c], mx);
+              const float alpha = mn == -INFINITY ? 1.0f : ex2_approx(m1[nt][c] - mn);
+              m1[nt][c] = mn;
+              l[nt][c] *= alpha;
+#pragma unroll
+              for (int x = 0; x < NT; ++x) {
+                acc[x][nt][c] *= alpha;
+                acc[x][nt][c + 2] *= alpha;
+              }
             }
-          }
-      }
-      // ---- weights, as the B operand of O^T = V^T P^T
-      uint32_t pf[NR][2];
-      if constexpr (I8) {
-        vs[0] *= down;
-        vs[1] *= down;
-      }
-#pragma unroll
-      for (int nt = 0; nt < NR; ++nt) {
-        const float u0 = m1[nt][0] == -INFINITY ? 0.0f : m1[nt][0], u1 = m1[nt][1] == -INFINITY ? 0.0f : m1[nt][1];
-        float e[4] = {ex2_approx(sc[nt][0] - u0), ex2_approx(sc[nt][1] - u1), ex2_approx(sc[nt][2] - u0),
-                      ex2_approx(sc[nt][3] - u1)};
-        l[nt][0] += e[0] + e[2];
-        l[nt][1] += e[1] + e[3];
-        if constexpr (I8) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            e[c] *= vs[c >> 1];
-            if (!whole && !((seen >> (4 * nt + c)) & 1u)) e[c] = 0.0f;  // the scale may be a NaN
-          }
         }
-        pf[nt][0] = movmatrix(pack2<M>(e[0], e[1]));
-        pf[nt][1] = movmatrix(pack2<M>(e[2], e[3]));
+        // ---- weights
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt) {
+          const float u0 = m1[nt][0] == -INFINITY ? 0.0f : m1[nt][0], u1 = m1[nt][1] == -INFINITY ? 0.0f : m1[nt][1];
+          const float e[4] = {ex2_approx(sc[nt][0] - u0), ex2_approx(sc[nt][1] - u1), ex2_approx(sc[nt][2] - u0),
+                              ex2_approx(sc[nt][3] - u1)};
+          l[nt][0] += e[0] + e[2];
+          l[nt][1] += e[1] + e[3];
+          pf[nt][0] = movmatrix(pack2<M>(e[0], e[1]));
+          pf[nt][1] = movmatrix(pack2<M>(e[2], e[3]));
+        }
+      } else {
+        // ---- exponentials and weights; where one outgrew its range, new maxima and units, and once more
+        float e[NR][4], w8[NR][4];
+        auto weigh = [&] {
+          bool grow = false;
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              const float2 a = fadd2(make_float2(sc[nt][2 * x], sc[nt][2 * x + 1]), make_float2(-m1[nt][0], -m1[nt][1]));
+              const float2 y = make_float2(ex2_approx(a.x), ex2_approx(a.y));
+              const float2 z = fmul2(fmul2(y, make_float2(vs[x], vs[x])), make_float2(down[nt][0], down[nt][1]));
+              e[nt][2 * x] = y.x; e[nt][2 * x + 1] = y.y;
+              w8[nt][2 * x] = z.x; w8[nt][2 * x + 1] = z.y;
+            }
+            if (!whole) {
+#pragma unroll
+              for (int c = 0; c < 4; ++c)
+                if (!((seen >> (4 * nt + c)) & 1u)) w8[nt][c] = 0.0f;  // the scale may be a NaN
+            }
+            grow |= fmax3(fmaxf(fabsf(w8[nt][0]), fabsf(w8[nt][1])), fabsf(w8[nt][2]), fabsf(w8[nt][3])) > 16384.0f ||
+                    fmax3(fmaxf(e[nt][0], e[nt][1]), e[nt][2], e[nt][3]) > 1.152921504606847e18f;  // 2^60
+          }
+          return grow;
+        };
+        if (__builtin_expect(__any_sync(0xffffffffu, weigh()), 0)) {
+#pragma unroll
+          for (int nt = 0; nt < NR; ++nt)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float mx = fmaxf(sc[nt][c], sc[nt][c + 2]);
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+              const float mo = m1[nt][c], mn = fmaxf(mo, mx);
+              // fmaxf drops a NaN (of a scale that this row does not see: 0 * NaN)
+              float top = fmaxf(fmaxf(fabsf(ex2_approx(sc[nt][c] - mn) * vs[0]), fabsf(ex2_approx(sc[nt][c + 2] - mn) * vs[1])), 0.0f);
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              // the weights of before have shrunk by 2^(mn - mo), so may their unit
+              const int before = mo == kNoScore ? -126 : unit[nt][c] - (int)ceilf(fminf(mn - mo, 256.0f));
+              const int now = max(max(exponent(top), before), -126);
+              const float alpha = ex2_approx(mo - mn), move = ex2_approx((mo - mn) + (float)(unit[nt][c] - now));
+              m1[nt][c] = mn;
+              unit[nt][c] = now;
+              down[nt][c] = pow2(-now);
+              l[nt][c] *= alpha;
+#pragma unroll
+              for (int x = 0; x < NT; ++x) {
+                acc[x][nt][c] *= move;
+                acc[x][nt][c + 2] *= move;
+              }
+            }
+          (void)weigh();
+        }
+#pragma unroll
+        for (int nt = 0; nt < NR; ++nt) {
+          const float2 sum = fadd2(make_float2(l[nt][0], l[nt][1]), fadd2(make_float2(e[nt][0], e[nt][1]), make_float2(e[nt][2], e[nt][3])));
+          l[nt][0] = sum.x;
+          l[nt][1] = sum.y;
+          pf[nt][0] = movmatrix(pack2<M>(w8[nt][0], w8[nt][1]));
+          pf[nt][1] = movmatrix(pack2<M>(w8[nt][2], w8[nt][3]));
+        }
       }
       // ---- O^T += V^T P^T over this warp's 16 keys
       if constexpr (!I8) {
@@ -673,7 +730,7 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
           float* x = ml + (warp * C::ROWS + 8 * nt + 2 * t + c) * 4;
           x[0] = m1[nt][c];
           x[1] = l[nt][c];
-          x[2] = I8 ? m1[nt][c] + unit_v : m1[nt][c];
+          if constexpr (I8) x[2] = (float)unit[nt][c];
         }
       }
     asm volatile("bar.sync 1, %0;" ::"n"(kDecWarps * 32) : "memory");
@@ -682,10 +739,18 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
         const int row = 8 * nt + 2 * t + c;
-        float mo = -INFINITY;
+        float ms = I8 ? kNoScore : -INFINITY, f;
 #pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) mo = fmaxf(mo, ml[(w * C::ROWS + row) * 4 + 2]);
-        const float f = ex2_approx((I8 ? m1[nt][c] + unit_v : m1[nt][c]) - (mo == -INFINITY ? 0.0f : mo));
+        for (int w = 0; w < kDecWarps; ++w) ms = fmaxf(ms, ml[(w * C::ROWS + row) * 4]);
+        if constexpr (I8) {
+          float eo = -126.0f;
+#pragma unroll
+          for (int w = 0; w < kDecWarps; ++w)
+            eo = fmaxf(eo, unit_under(ml[(w * C::ROWS + row) * 4], ml[(w * C::ROWS + row) * 4 + 2], ms));
+          f = ex2_approx((m1[nt][c] - ms) + ((float)unit[nt][c] - eo));
+        } else {
+          f = ex2_approx(m1[nt][c] - (ms == -INFINITY ? 0.0f : ms));
+        }
         float* dst = red + (warp * C::ROWS + row) * C::RED_STRIDE;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -705,29 +770,28 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
       const int row = idx / (D / 4), c4 = idx % (D / 4);
       if (row >= rows) continue;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float ms = -INFINITY, mo = -INFINITY, sum = 0.0f;
+      float ms = I8 ? kNoScore : -INFINITY, eo = -126.0f, sum = 0.0f;
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
         const float4 v = *reinterpret_cast<const float4*>(red + (w * C::ROWS + row) * C::RED_STRIDE + c4 * 4);
         o.x += v.x; o.y += v.y; o.z += v.z; o.w += v.w;
         ms = fmaxf(ms, ml[(w * C::ROWS + row) * 4]);
-        mo = fmaxf(mo, ml[(w * C::ROWS + row) * 4 + 2]);
       }
       const float use = ms == -INFINITY ? 0.0f : ms;
 #pragma unroll
       for (int w = 0; w < kDecWarps; ++w) {
         const float* y = ml + (w * C::ROWS + row) * 4;
         sum = fmaf(y[1], ex2_approx(y[0] - use), sum);
+        if constexpr (I8) eo = fmaxf(eo, unit_under(y[0], y[2], ms));
       }
       if (begins && ends) {
-        // INT8: the outputs' unit is their own
-        const float inv = sum == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - use) / sum : 1.0f / sum);
+        const float inv = sum == 0.0f ? 0.0f : (I8 ? pow2((int)eo) : 1.0f) / sum;
         const int fr = mt * C::ROWS + row, tok = fr / p.G, hd = fr - tok * p.G;
         T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(h * p.G + hd) * p.o_sh + c4 * 4;
         *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
       } else {
         *reinterpret_cast<float4*>(p.part + ((int64_t)slot * C::ROWS + row) * D + c4 * 4) = o;
-        if (c4 == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * C::ROWS + row) * 4) = make_float4(ms, sum, mo, 0.0f);
+        if (c4 == 0) *reinterpret_cast<float4*>(p.part_ml + (slot * C::ROWS + row) * 4) = make_float4(ms, sum, I8 ? eo : 0.0f, 0.0f);
       }
     }
     if (begins && !ends) cut = make_int4(seg.b, h, mt, (int)((ts.count - n + per - 1) / per));
@@ -753,7 +817,8 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
   const int fr = d.z * ROWS + row;
   if (fr >= sq.n * p.G) return;
   const int tok = fr / p.G, hd = fr - tok * p.G;
-  float o[E], ms = -INFINITY, l = 0.0f, mo = -INFINITY;
+  // eo: INT8, the outputs are in units of 2^(ms + eo)
+  float o[E], ms = I8 ? kNoScore : -INFINITY, l = 0.0f, eo = -126.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
 #pragma unroll 4
@@ -770,11 +835,15 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
       v[0] = y.x; v[1] = y.y;
     }
     const float mn = fmaxf(ms, x.x), us = mn == -INFINITY ? 0.0f : mn;
-    l = fmaf(l, ex2_approx(ms - us), x.y * ex2_approx(x.x - us));
+    float fa = ex2_approx(ms - us), fb = ex2_approx(x.x - us);
+    l = fmaf(l, fa, x.y * fb);
+    if constexpr (I8) {
+      const float en = fmaxf(unit_under(ms, eo, mn), unit_under(x.x, x.z, mn));
+      fa = ex2_approx((ms - mn) + (eo - en));
+      fb = ex2_approx((x.x - mn) + (x.z - en));
+      eo = en;
+    }
     ms = mn;
-    const float on = fmaxf(mo, x.z), uo = on == -INFINITY ? 0.0f : on;
-    const float fa = ex2_approx(mo - uo), fb = ex2_approx(x.z - uo);
-    mo = on;
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(o[e], fa, v[e] * fb);
   }
@@ -783,28 +852,31 @@ __global__ void __launch_bounds__(kCombineThreads) paged_combine_kernel(const De
   if (lane == 0) {
     s_ml[warp][0] = ms;
     s_ml[warp][1] = l;
-    s_ml[warp][2] = mo;
+    s_ml[warp][2] = eo;
   }
   __syncthreads();
   if (warp != 0) return;
-  ms = mo = -INFINITY;
+  ms = I8 ? kNoScore : -INFINITY;
+  eo = -126.0f;
 #pragma unroll
-  for (int w = 0; w < W; ++w) {
-    ms = fmaxf(ms, s_ml[w][0]);
-    mo = fmaxf(mo, s_ml[w][2]);
+  for (int w = 0; w < W; ++w) ms = fmaxf(ms, s_ml[w][0]);
+  if constexpr (I8) {
+#pragma unroll
+    for (int w = 0; w < W; ++w) eo = fmaxf(eo, unit_under(s_ml[w][0], s_ml[w][2], ms));
   }
   l = 0.0f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.0f;
-  const float us = ms == -INFINITY ? 0.0f : ms, uo = mo == -INFINITY ? 0.0f : mo;
+  const float us = ms == -INFINITY ? 0.0f : ms;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    l = fmaf(s_ml[w][1], ex2_approx(s_ml[w][0] - us), l);
-    const float f = ex2_approx(s_ml[w][2] - uo);
+    float f = ex2_approx(s_ml[w][0] - us);
+    l = fmaf(s_ml[w][1], f, l);
+    if constexpr (I8) f = ex2_approx((s_ml[w][0] - ms) + (s_ml[w][2] - eo));
 #pragma unroll
     for (int e = 0; e < E; ++e) o[e] = fmaf(s_o[w][lane * E + e], f, o[e]);
   }
-  const float inv = l == 0.0f ? 0.0f : (I8 ? ex2_approx(mo - us) / l : 1.0f / l);
+  const float inv = l == 0.0f ? 0.0f : (I8 ? pow2((int)eo) : 1.0f) / l;
   T* dst = static_cast<T*>(p.o) + (int64_t)(sq.base + tok) * p.o_st + (int64_t)(d.y * p.G + hd) * p.o_sh + lane * E;
   if constexpr (E == 4)
     *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(o[0] * inv, o[1] * inv), pack2<T>(o[2] * inv, o[3] * inv));
