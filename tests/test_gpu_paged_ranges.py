@@ -140,3 +140,26 @@ def test_wide_scales_beside_plain_sequences(n):
     o = run(c)
     assert worst(c, o) <= 1
     assert torch.equal(o, run(c))
+
+
+@pytest.mark.parametrize("n", [1, 4, 100])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_key_that_is_not_finite(n, bad, dim):
+    """A key row with an infinity or a NaN is held as NaN: queries that see it get NaN, the others do not notice."""
+    for at in (3, 40, 41 + n - 1):
+        c = make_case(DEV, new=[n], past=[41], hq=4, hkv=2, dim=dim, page=16, dtype=F16, storage="int8", seed=11)
+        cache = cache_of(c)
+        one = torch.randn(1, 2, dim, device=DEV).half()
+        k = one.clone()
+        k[0, :, 5] = bad
+        i32 = dict(dtype=torch.int32, device=DEV)
+        cache.append(k, one, c["table"], torch.tensor([at + 1], **i32))
+        assert bool(cache.gather(c["table"], torch.tensor([at + 1], **i32))[0].isnan().all())
+        o = run(c)
+        unseen = max(at - 41, 0)  # rows before the key
+        assert bool(o[unseen:].isnan().all())
+        # to the bound's arithmetic the key does not exist for rows before it
+        c["kw"]["k_scale"].nan_to_num_(nan=0.0, posinf=0.0)
+        if unseen:
+            assert worst(c, o, rows=unseen) <= 1

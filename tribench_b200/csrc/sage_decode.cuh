@@ -527,7 +527,11 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
         }
         const float* scales = reinterpret_cast<const float*>(smem + s * C::STAGE + 2 * C::TILE);
         const int at = k_warp + g;
-        const float ks0 = scales[at], ks1 = scales[at + 8];
+        // an infinite scale (of a row that holds an infinity) becomes NaN: its codes are 0, but what is left of
+        // 2^24 S' - 128 sum(q) after rounding would give it a sign
+        float ks0 = scales[at], ks1 = scales[at + 8];
+        ks0 += ks0 - ks0;
+        ks1 += ks1 - ks1;
         vs[0] = scales[C::SCALES / 4 + at];
         vs[1] = scales[C::SCALES / 4 + at + 8];
 #pragma unroll
