@@ -163,3 +163,13 @@ def test_a_key_that_is_not_finite(n, bad, dim):
         c["kw"]["k_scale"].nan_to_num_(nan=0.0, posinf=0.0)
         if unseen:
             assert worst(c, o, rows=unseen) <= 1
+
+
+@pytest.mark.parametrize("n", [1, 4, 100])
+@pytest.mark.parametrize("log2", [-110, -60, 60, 100, 118])
+def test_queries_of_any_size(n, log2):
+    """Queries far from 1 with keys that make up for it: scores are as usual."""
+    c = make_case(DEV, new=[n], past=[200], hq=4, hkv=2, dim=128, page=16, dtype=BF16, storage="int8", seed=12)
+    c["q"] = (c["q"].double() * 2.0 ** log2).to(BF16)
+    c["kw"]["k_scale"] *= 2.0 ** -log2
+    assert worst(c, run(c)) <= 1

@@ -196,6 +196,9 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
   constexpr int KS = D / 16;   // k-steps of q . K
   constexpr int NT = D / 16;   // 16-channel tiles of the output
   constexpr float LAZY = 8.0f;
+  // INT8: the part of the subnormals' 2^24 that goes to the scales of the keys, as 2^24 times a large query's unit
+  // would leave fp32
+  constexpr float K_UNIT = 1048576.0f;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::OFF_BAR);
@@ -446,8 +449,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
 #pragma unroll
         for (int c = 0; c < 2; ++c) {  // row 2 t + c is that of lanes 4 (2 t + c)
           const float ar = __shfl_sync(0xffffffffu, a, 4 * (2 * t + c)), sr = __shfl_sync(0xffffffffu, sum, 4 * (2 * t + c));
-          qa[nt][c] = ar * 16777216.0f;
-          qb[nt][c] = -128.0f * sr * ar;
+          qa[nt][c] = ar * (16777216.0f / K_UNIT);
+          qb[nt][c] = (-128.0f / K_UNIT * sr) * ar;
         }
       }
     }
@@ -530,8 +533,8 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
         // an infinite scale (of a row that holds an infinity) becomes NaN: its codes are 0, but what is left of
         // 2^24 S' - 128 sum(q) after rounding would give it a sign
         float ks0 = scales[at], ks1 = scales[at + 8];
-        ks0 += ks0 - ks0;
-        ks1 += ks1 - ks1;
+        ks0 = fmaf(ks0, K_UNIT, ks0 - ks0);
+        ks1 = fmaf(ks1, K_UNIT, ks1 - ks1);
         vs[0] = scales[C::SCALES / 4 + at];
         vs[1] = scales[C::SCALES / 4 + at + 8];
 #pragma unroll
