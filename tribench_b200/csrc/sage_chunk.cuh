@@ -48,6 +48,7 @@
 
 #include "sage_attn.cuh"
 #include "sage_decode.cuh"
+#include "sage_inflight.cuh"
 
 namespace sage {
 
@@ -92,7 +93,7 @@ struct ChunkCfg {
   static constexpr int OUT_BYTES = 32 * OUT_CH * 2;          // per softmax warp: 32 rows of them
   static constexpr int OFF_OUT = OFF_V + NS * TILE;
   static constexpr int OFF_BAR = OFF_OUT + 8 * OUT_BYTES;
-  static constexpr int NUM_BARS = 3 + 7 * NS + 12;
+  static constexpr int NUM_BARS = 4 + 7 * NS + 12;
   static constexpr int OFF_MISC = OFF_BAR + NUM_BARS * 8;
   static constexpr int OFF_WALK = (OFF_MISC + 8 + 15) / 16 * 16;  // where each warp is in the piece
   static constexpr int WALK_BYTES = 80;
@@ -101,7 +102,8 @@ struct ChunkCfg {
   static constexpr int SMEM_BYTES = 1024 + OFF_EXP + (I8 ? 16 : 0);
   static_assert(SMEM_BYTES <= 227 * 1024 && SMEM_BYTES > 114 * 1024, "one CTA per SM");
   // 256 softmax and 128 other threads share 384 x 168 registers; a converter keeps 32 registers of loads in flight
-  static constexpr int REGS_SOFTMAX = I8 ? 208 : 216, REGS_OTHER = I8 ? 88 : 72;
+  // (two chunks of 1024 over 7168: head_dim 64 335 us with 104 registers, 367 with 88; 128 364 and 374 the other way)
+  static constexpr int REGS_SOFTMAX = I8 ? (D == 64 ? 200 : 208) : 216, REGS_OTHER = I8 ? (D == 64 ? 104 : 88) : 72;
   static_assert(256 * REGS_SOFTMAX + 128 * REGS_OTHER <= 384 * 168, "register split");
   static constexpr uint32_t QK_LAYOUT = kLayoutSW128, QK_SBO = 1024;
   static constexpr int QK_STEPS = D / 16;
@@ -361,6 +363,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   uint64_t* bar_sc = bar_pvdone + 2;    // [stage] INT8: the tile's scales are in place
   uint64_t* bar_kraw = bar_sc + C::NS;  // [stage] INT8: K's codes landed (V's: bar_vraw)
   uint64_t* bar_qraw = bar_kraw + C::NS;  // bf16 queries landed, to be converted by the softmax threads
+  uint64_t* bar_mma = bar_qraw + 1;       // after a wait ran out: every product has run
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::OFF_MISC);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + C::OFF_MISC + 4);
   const uint32_t warp = warp_id(), lane = lane_id();
@@ -369,6 +372,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(bar_q, Q_CONV ? 256 : 1);
     mbar_init(bar_qraw, 1);
+    mbar_init(bar_mma, 1);
     mbar_init(bar_qfree, 1);
     for (int s = 0; s < C::NS; ++s) {
       mbar_init(bar_vraw + s, 1);
@@ -438,6 +442,10 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     seen(&hi, &lo);
     return key0 + 128 > hi || (key0 < lo && key0 + 128 > p.sinks);
   };
+
+    // what this warp has issued, for the case that a wait runs out
+    int tiles_k = 0, tiles_v = 0, segments = 0;
+    ValueCopies value_copies;
 
     // the segment's queries: one box per query tile and 64 channels
     auto load_queries = [&] {
@@ -564,7 +572,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       // ------------------------------------------------------------ TMA producer
       // boxes of K, and of V: one per page and 128-byte atom (INT8: per page, into the slot's upper half)
       const int boxes = I8 ? ppt : ppt * C::ATOMS;
-      int it = 0;
+      int it = 0, k_ahead = 0;  // k_ahead: gave up between a tile's K and V
       bool ok = true;
       for (int seg = 0; w.more() && ok; step(), ++seg) {
         if constexpr (I8) {  // the queries too: warp 10 converts
@@ -573,6 +581,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (!ok) break;
           if (lane == 0) load_queries();
           __syncwarp();
+          segments = seg + 1;
         }
         const int kvh = w.head / p.parts;
         int next = page_of(0);
@@ -586,14 +595,18 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             const int sub = lane % ppt, atom = lane / ppt;
             const int id = __shfl_sync(0xffffffffu, ids, (j - j0) * ppt + sub);
             const int dst = s * C::TILE + (I8 ? C::TILE / 2 + sub * rows * D : atom * (128 * 128) + sub * rows * 128);
-            uint64_t* vbar = (I8 || ragged(key0) ? bar_vraw : bar_vfull) + s;
+            const bool raw = I8 || ragged(key0);
+            uint64_t* vbar = (raw ? bar_vraw : bar_vfull) + s;
 #pragma unroll
             for (int isv = 0; isv < 2; ++isv) {
               if (ok && it >= C::NS)
                 ok = mbar_wait((isv ? bar_vempty : bar_kempty) + s, ((it / C::NS) - 1) & 1, abort_flag, kDevTimeoutProducer,
                                p.wait_limit_ns);
               ok = __all_sync(0xffffffffu, ok);
-              if (!ok) break;
+              if (!ok) {
+                k_ahead = isv;
+                break;
+              }
               uint64_t* bar = isv ? vbar : (I8 ? bar_kraw : bar_kfull) + s;
               if (lane == 0) mbar_arrive_expect_tx(bar, I8 ? C::TILE / 2 : C::TILE);
               __syncwarp();
@@ -601,15 +614,12 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
                 tma_load_4d(smem + (isv ? C::OFF_V : C::OFF_K) + dst, isv ? &tmV : &tmK, bar, atom * 64, y, kvh, id);
             }
             if (!ok) break;
+            if constexpr (!I8) value_copies.note(s, it / C::NS, raw);
           }
         }
       }
-      if (!ok) {  // gave up: wait (bounded) for the copies of K in flight (those of V were issued with them)
-        for (int j = max(0, it - C::NS); j < it; ++j) {
-          volatile int none = 0;
-          (void)mbar_wait((I8 ? bar_kraw : bar_kfull) + j % C::NS, (j / C::NS) & 1, &none, kDevTimeoutProducer, p.wait_limit_ns);
-        }
-      }
+      tiles_v = it;
+      tiles_k = it + k_ahead;
     } else if (warp == 9) {
       // ------------------------------------------------------------ MMA issuer
       if (elect_one()) {
@@ -701,6 +711,7 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           if (seg > 0) ok = mbar_wait(bar_qfree, (seg - 1) & 1, abort_flag, kDevTimeoutProducer, p.wait_limit_ns);
           if (!ok) break;
           load_queries();
+          segments = seg + 1;
         }
       }
     } else {
@@ -732,12 +743,34 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
     }
     // every warp leaves through barrier 2; the MMA warp frees TMEM after all have arrived
     tc_fence_before();
+    if (warp == 11) {
+      asm volatile("bar.arrive 2, %0;" ::"n"(kChunkThreads) : "memory");
+      return;
+    }
+    __syncwarp();
+    asm volatile("bar.sync 2, %0;" ::"n"(kChunkThreads) : "memory");
+    if (*abort_flag) {
+      // A wait ran out, so what this warp issued may still be on its way: wait for it, again within the limit.
+      auto landed = [&](uint64_t* bar, uint32_t phase) {
+        volatile int none = 0;
+        (void)mbar_wait(bar, phase, &none, kDevTimeoutProducer, p.wait_limit_ns);
+      };
+      const CopyLedger k = ring_copies(tiles_k, C::NS), v = I8 ? ring_copies(tiles_v, C::NS) : value_copies.raw;
+      for (int s = 0; s < C::NS; ++s) {
+        if (k.pending(s)) landed((I8 ? bar_kraw : bar_kfull) + s, k.phase(s));
+        if (v.pending(s)) landed(bar_vraw + s, v.phase(s));
+        if (value_copies.full.pending(s)) landed(bar_vfull + s, value_copies.full.phase(s));
+      }
+      if (segments > 0) landed(Q_CONV ? bar_qraw : bar_q, (segments - 1) & 1);
+      if (warp == 9 && elect_one()) {
+        umma_commit(bar_mma);
+        landed(bar_mma, 0);
+      }
+      __syncwarp();
+    }
     if (warp == 9) {
-      asm volatile("bar.sync 2, %0;" ::"n"(kChunkThreads) : "memory");
       tc_fence_after();
       tmem_dealloc(tmem_base, 512);
-    } else {
-      asm volatile("bar.arrive 2, %0;" ::"n"(kChunkThreads) : "memory");
     }
   } else {
     // ------------------------------------------------------------ softmax warpgroups

@@ -330,12 +330,11 @@ __global__ void __launch_bounds__(kDecThreads, DecodeCfg<D, I8, NR>::CTAS)
       rem += n;
       left -= n;
     }
-    if (!ok) {
-      // gave up: wait (bounded) for the copies in flight before the block's shared memory goes
-      for (int j = max(0, it - C::NS); j < it; ++j) {
-        volatile int none = 0;
-        (void)mbar_wait(full + j % C::NS, (j / C::NS) & 1, &none, 1, p.wait_limit_ns);
-      }
+    // The last copies must have landed before the block's shared memory goes, whoever gave up meanwhile (the
+    // abort flag does not end these waits, their limit does).
+    for (int j = max(0, it - C::NS); j < it; ++j) {
+      volatile int none = 0;
+      (void)mbar_wait(full + j % C::NS, (j / C::NS) & 1, &none, 1, p.wait_limit_ns);
     }
     return;
   }
