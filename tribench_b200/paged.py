@@ -106,7 +106,18 @@ class PagedKVCache:
     before they are quantised and added when they are read back, the cache's form of the smoothing of
     run_sage_attn: keys share large channel offsets that would use up the codes' range, and a constant
     offset of all keys does not change attention. It must stay the same for the cache's life.
+
+    The tensors and sizes are fixed: the calls use the addresses of construction, so neither the
+    attributes nor the tensors' storages can be exchanged (their contents can).
     """
+
+    _FIXED = frozenset(("k", "v", "k_scale", "v_scale", "k_mean", "dtype", "device", "tensor_layout", "storage", "num_pages",
+                        "heads_kv", "page_size", "head_dim"))
+
+    def __setattr__(self, name, value):
+        if name in self._FIXED and "_c" in self.__dict__:
+            raise AttributeError(f"PagedKVCache.{name} is fixed: make another cache for other tensors")
+        object.__setattr__(self, name, value)
 
     def __init__(self, k, v, *, k_scale=None, v_scale=None, k_mean=None, dtype=None, tensor_layout="HND"):
         _check_tensor("k", k)
