@@ -193,9 +193,9 @@ enum class PagedRoute { kFew, kMany, kBoth };
 // and the others have few on average (single tokens beside a chunk), both kernels run, each on the
 // sequences of its kind; else the largest decides.
 PagedRoute paged_route(const sage_paged_cache* c, int64_t G, int64_t batch, int64_t total_q, int64_t max_seqlen_q) {
-  const int64_t few = few_rows(c);
-  if (max_seqlen_q * G <= few) return PagedRoute::kFew;
-  const bool mixed = batch >= kMixedBatch && (total_q - std::min(max_seqlen_q, total_q)) * G <= few * (batch - 1);
+  const int64_t few = few_rows(c), largest = std::min(max_seqlen_q, total_q);  // a bound may be anything above
+  if (largest * G <= few) return PagedRoute::kFew;
+  const bool mixed = batch >= kMixedBatch && (total_q - largest) * G <= few * (batch - 1);
   return mixed ? PagedRoute::kBoth : PagedRoute::kMany;
 }
 
