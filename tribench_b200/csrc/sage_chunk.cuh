@@ -21,24 +21,31 @@
 // INT8 cache: helper warps turn the codes into fp16 tiles (exact) in shared memory, in the layout the
 // TMA load would give, and the scales stay out of the products: scores are multiplied by k_scale per
 // column in fp32, P by v_scale before it is rounded to fp16, in units of a power of two 2^E. Two ways:
-// - The tile's visible scales (other than 0) span less than 2^7, as those of most models do: one E for
-//   the tile, 2^E <= v_scale < 2^(E + 7), kept from tile to tile while it fits, else moved and O rescaled.
-//   P < 2^8 * 2^7 stays inside fp16, and what it loses below 2^(E - 25) is at most 2^-25 of v_scale.
+// - The tile's visible scales (other than 0) span less than 2^11, the usual case: one E for the tile,
+//   2^E <= v_scale < 2^(E + 11), kept from tile to tile while it fits, else moved and O rescaled. P < 2^4 *
+//   2^11 stays inside fp16 (hence a maximum less lazy than 16 bit's 2^8), and what it loses below 2^(E - 25)
+//   is at most 2^-25 of v_scale.
 // - They span more, or E would move by more than 2^30 within a segment: E per query row, 2^E <= the
 //   largest P v_scale that the row has met, from the products themselves, for this tile and the rest of
 //   the segment. A key weighs by what it contributes to the row, whatever scales other keys have. The
-//   softmax loop stays the same: E goes into the exponent, and out of the sum of the tile.
+//   softmax loop stays the same: E goes into the exponent, and out of the sum of the tile. What finds it
+//   is a pass of its own over S (random scales over 2^20, the chunks below, fp16: 534 us; single
+//   tokens have no such case).
 // bf16 queries are brought to fp16 by a power of two per row.
 //
 // Code size counts: the softmax's and the converters' loops run side by side on the same instruction
-// cache, and unrolled whole (22 KB of converter) the INT8 kernel took 475 us where this one takes 343
+// cache, and unrolled whole (22 KB of converter) the INT8 kernel took 475 us where the loop took 343
 // (two chunks of 1024 over 7168, 32/8 heads, head_dim 128). For the same reason every exponential is
 // MUFU.ex2: the polynomial share that sage_attn.cuh computes on the FMA pipe costs more here (12 of 32
 // columns: 16 bit 243 -> 231 us, INT8 540 -> 475 us without).
 //
-// Measured (B200, two chunks of 1024 tokens over 7168, 32/8 heads, head_dim 128): bf16 227 us, 1136
-// TFLOP/s; INT8 (fp16) 341 us; head_dim 64: 194 us (663 TFLOP/s) and 308 us. A tile of 128 keys takes
-// about 4100 clk, the chain S -> softmax -> P V -> next S of the two query tiles in turn.
+// P is rounded to the operand type as in sage_decode.cuh; scores, sums and outputs are fp32.
+//
+// Measured (B200, two chunks of 1024 tokens over 7168, 32/8 heads, head_dim 128, calls back to back): bf16 226 to
+// 232 us, 1111 to 1140 TFLOP/s; INT8 344 us (fp16) and 340 us (bf16); head_dim 64: 195 to 207 us (623 to 661
+// TFLOP/s), INT8 333 us (fp16) and 332 us (bf16). Chunks of 512 and 1024 over 8192 and 16384, bf16: 364 to 371 us,
+// 954 to 974 TFLOP/s. A tile of 128 keys takes about 4100 clk, the chain S -> softmax -> P V -> next S of the two
+// query tiles in turn.
 //
 // Warps: 0-7 softmax (two warpgroups), 8 TMA producer of K and V, 9 MMA issuer, 10 loads the next
 // segment's queries as soon as the last Q K^T of this one has run, 11 puts zeros over rows of V that no
@@ -98,12 +105,15 @@ struct ChunkCfg {
   static constexpr int OFF_WALK = (OFF_MISC + 8 + 15) / 16 * 16;  // where each warp is in the piece
   static constexpr int WALK_BYTES = 80;
   static constexpr int OFF_SCALE = (OFF_WALK + 12 * WALK_BYTES + 15) / 16 * 16;  // INT8: per stage k_scale, v_scale 2^-E
-  static constexpr int OFF_EXP = OFF_SCALE + (I8 ? NS * 1024 : 0);               // and E
+  static constexpr int OFF_LOG = OFF_SCALE + (I8 ? NS * 1024 : 0);               // log2 v_scale, for units of the rows
+  static constexpr int OFF_EXP = OFF_LOG + (I8 ? NS * 512 : 0);                  // and E
   static constexpr int SMEM_BYTES = 1024 + OFF_EXP + (I8 ? 16 : 0);
   static_assert(SMEM_BYTES <= 227 * 1024 && SMEM_BYTES > 114 * 1024, "one CTA per SM");
-  // 256 softmax and 128 other threads share 384 x 168 registers; a converter keeps 32 registers of loads in flight
-  // (two chunks of 1024 over 7168: head_dim 64 335 us with 104 registers, 367 with 88; 128 364 and 374 the other way)
-  static constexpr int REGS_SOFTMAX = I8 ? (D == 64 ? 200 : 208) : 216, REGS_OTHER = I8 ? (D == 64 ? 104 : 88) : 72;
+  // 256 softmax and 128 other threads share 384 x 168 registers; a converter keeps 32 registers of loads in flight.
+  // Two chunks of 1024 over 7168, INT8: head_dim 64, fp16, 104 registers for the others 340 us, 120 347; bf16 120 339,
+  // 104 350, 88 393; head_dim 128, fp16, 88 364 us, 104 374.
+  static constexpr int REGS_OTHER = !I8 ? 72 : D == 128 ? 88 : std::is_same<T, M>::value ? 104 : 120;
+  static constexpr int REGS_SOFTMAX = (384 * 168 - 128 * REGS_OTHER) / 256;
   static_assert(256 * REGS_SOFTMAX + 128 * REGS_OTHER <= 384 * 168, "register split");
   static constexpr uint32_t QK_LAYOUT = kLayoutSW128, QK_SBO = 1024;
   static constexpr int QK_STEPS = D / 16;
@@ -117,11 +127,12 @@ struct ChunkCfg {
   static constexpr uint32_t FMT = std::is_same<M, __half>::value ? kFmtF16 : kFmtBF16;
   static constexpr uint32_t IDESC_QK = make_idesc(kFmtD_F32, FMT, FMT, 0, 0, BM, BN);
   static constexpr uint32_t IDESC_PV = make_idesc(kFmtD_F32, FMT, FMT, 0, 1, BM, D);
-  static constexpr float LAZY = 8.0f;
+  static constexpr float LAZY = I8 ? 4.0f : 8.0f;
 };
-// INT8, added to a tile's E where every row finds its own unit. E is then kRowRange below the largest scale so
-// far: the row's unit may be kRowRange + 1 above E and 2^kRowDepth below before an exponential leaves fp32.
-constexpr int kRowUnits = 1 << 20, kRowRange = 60, kRowDepth = 118;
+// INT8: the exponents that the scales of a tile of one E may differ by. kRowUnits is added to E where every row
+// finds its own unit; E is then kRowRange below the largest scale so far: the row's unit may be kRowRange + 1
+// above E and kRowDepth below before an exponential leaves fp32.
+constexpr int kUnitSpan = 10, kRowUnits = 1 << 20, kRowRange = 60, kRowDepth = 118;
 
 // ------------------------------------------------------------------ schedule
 __device__ __forceinline__ int chunk_blocks(const ChunkParams& p, const PagedSeq& sq) {
@@ -313,6 +324,12 @@ __device__ __forceinline__ void tma_load_3d(void* smem_dst, const CUtensorMap* m
       : "memory");
 }
 
+__device__ __forceinline__ float lg2_approx(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 // The lowest n bits (n may be anything).
 __device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
 
@@ -344,6 +361,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
   using C = ChunkCfg<D, I8, T>;
   using M = typename C::M;
   constexpr bool Q_CONV = I8 && std::is_same<T, __nv_bfloat16>::value;  // queries from bf16 to fp16
+  // How far the pass for units of the rows is unrolled: it hardly runs, but where it puts the code behind it in the
+  // instruction cache shows (two chunks of 1024 over 7168; rolled, by 2, whole: fp16 359, 365, 351 us, bf16 360, 350, 397)
+  constexpr int ROW_PASS = Q_CONV ? 2 : 4;
   const DecodeParams& p = cp.d;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -430,18 +450,17 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
       if constexpr (I8) shared_next();
       else own.next();
     };
-    // first key behind those that some query of the segment sees, and first of its window
-  auto seen = [&](int* hi, int* lo) {
-    const int first = w.it.len - w.it.n + w.first_tok(cp);
-    *hi = p.causal ? first + w.toks(cp) : w.it.len;
-    *lo = p.window ? first - p.window + 1 : 0;
-  };
-  // a tile that holds rows of V which no query of the block sees
-  auto ragged = [&](int key0) {
-    int hi, lo;
-    seen(&hi, &lo);
-    return key0 + 128 > hi || (key0 < lo && key0 + 128 > p.sinks);
-  };
+      auto seen = [&](int* hi, int* lo) {
+      const int first = w.it.len - w.it.n + w.first_tok(cp);
+      *hi = p.causal ? first + w.toks(cp) : w.it.len;
+      *lo = p.window ? first - p.window + 1 : 0;
+    };
+    // a tile that holds rows of V which no query of the block sees
+    auto ragged = [&](int key0) {
+      int hi, lo;
+      seen(&hi, &lo);
+      return key0 + 128 > hi || (key0 < lo && key0 + 128 > p.sinks);
+    };
 
     // what this warp has issued, for the case that a wait runs out
     int tiles_k = 0, tiles_v = 0, segments = 0;
@@ -523,15 +542,15 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
               top = max(top, f);
               low = min(low, f ? f : 255u);
             }
-            const bool fits = has_unit && !row_units && (int)low >= e + 127 && (int)top <= e + 133;
+            const bool fits = has_unit && !row_units && (int)low >= e + 127 && (int)top <= e + 127 + kUnitSpan;
             if (!__all_sync(0xffffffffu, fits)) {
               top = __reduce_max_sync(0xffffffffu, top);
               low = __reduce_min_sync(0xffffffffu, low);
               const int t_hi = (int)top - 127, t_lo = (int)low - 127;
-              if (top == 255u || (top && t_hi - t_lo > 6)) {
+              if (top == 255u || (top && t_hi - t_lo > kUnitSpan)) {
                 row_units = true;
-              } else if (top && (!has_unit || t_lo < e || t_hi > e + 6)) {
-                e = min(max(t_lo - (6 - (t_hi - t_lo)) / 2, -126), 121);
+              } else if (top && (!has_unit || t_lo < e || t_hi > e + kUnitSpan)) {
+                e = min(max(t_lo - (kUnitSpan - (t_hi - t_lo)) / 2, -126), 121);
                 if (!has_unit) e_first = e;
                 has_unit = true;
                 row_units |= e > e_first + 30 || e < e_first - 30;
@@ -543,6 +562,9 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
             float4* sc = reinterpret_cast<float4*>(smem + C::OFF_SCALE + s * 1024);
             sc[lane] = make_float4(k4[0], k4[1], k4[2], k4[3]);
             sc[32 + lane] = make_float4(v4[0] * down, v4[1] * down, v4[2] * down, v4[3] * down);
+            if (row_units)
+              reinterpret_cast<float4*>(smem + C::OFF_LOG + s * 512)[lane] =
+                  make_float4(lg2_approx(fabsf(v4[0])), lg2_approx(fabsf(v4[1])), lg2_approx(fabsf(v4[2])), lg2_approx(fabsf(v4[3])));
             if (lane == 0) reinterpret_cast<int*>(smem + C::OFF_EXP)[s] = row_units ? unit + kRowUnits : unit;
             __syncwarp();
             if (lane == 0) mbar_arrive(bar_sc + s);
@@ -846,36 +868,38 @@ __global__ void __launch_bounds__(kChunkThreads, 1)
           const int e_tile = *reinterpret_cast<const int*>(smem + C::OFF_EXP + 4 * s);
           int e = e_tile;
           if (e_tile >= kRowUnits / 2) {
-            // Rare, and kept out of the code below: the row's unit, from its largest product, in two passes
-            // over S (32 columns at a time, from TMEM): the maximum, then the products.
+            // Rare, and kept out of the code below: the row's unit, from its largest product, by a pass over S
+            // (32 columns at a time, from TMEM).
             const int et = e_tile - kRowUnits;
-            float m = m_run, top = 0.0f;
-#pragma unroll 1
-            for (int c0 = 0; c0 < 256; c0 += 32) {
-              const int k0 = c0 & 127;
+            const uint32_t logs = smem_u32(smem + C::OFF_LOG) + s * 512;
+            float mx = -INFINITY, mo = -INFINITY;  // largest score (unscaled), largest log2 of a product
+#pragma unroll ROW_PASS
+            for (int c0 = 0; c0 < 128; c0 += 32) {
               uint32_t sr[32];
-              tmem_ld32_sync(s_tmem + k0, sr);
-              const float use = m == -INFINITY ? 0.0f : m;
+              tmem_ld32_sync(s_tmem + c0, sr);
+              const uint32_t vis = low_bits(up - c0) & (~low_bits(down - c0) | low_bits(sk - c0));
 #pragma unroll
               for (int c = 0; c < 32; c += 4) {
-                float2 ks[2], vs[2];
-                ld_shared_f4(scales + 4 * (k0 + c), ks);
-                ld_shared_f4(scales + 512 + 4 * (k0 + c), vs);
-                const float k4[4] = {ks[0].x, ks[0].y, ks[1].x, ks[1].y}, v4[4] = {vs[0].x, vs[0].y, vs[1].x, vs[1].y};
+                float2 ks[2], lg[2];
+                ld_shared_f4(scales + 4 * (c0 + c), ks);
+                ld_shared_f4(logs + 4 * (c0 + c), lg);
 #pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                  const int at = k0 + c + x;
-                  if (at < up && (at >= down || at < sk)) {
-                    const float b = __uint_as_float(sr[c + x]) * k4[x] * scale;
-                    if (c0 < 128) m = fmaxf(m, b);
-                    else top = fmaxf(top, fabsf(ex2_approx(b - use) * v4[x]));
-                  }
+                for (int x = 0; x < 2; ++x) {
+                  const int i = c + 2 * x;
+                  float2 b = fmul2(make_float2(__uint_as_float(sr[i]), __uint_as_float(sr[i + 1])), ks[x]);
+                  if (!((vis >> i) & 1u)) b.x = -INFINITY;
+                  if (!((vis >> (i + 1)) & 1u)) b.y = -INFINITY;
+                  const float2 y = ffma2(b, make_float2(scale, scale), lg[x]);
+                  mx = fmax3(mx, b.x, b.y);
+                  mo = fmax3(mo, y.x, y.y);
                 }
               }
             }
+            const float m = fmaxf(m_run, mx * scale);
+            const int top = mo == -INFINITY ? -126 : (int)floorf(fmaxf(mo - m, -126.0f));
             // the weights of before have shrunk by 2^(m - m_run), so may their unit
             const int before = m_run == -INFINITY ? -126 : e_run - (int)ceilf(fminf(m - m_run, 256.0f));
-            e = min(max(max(top > 0.0f ? exponent(top) + et : -126, before), max(et - kRowDepth, -126)), 121);
+            e = min(max(max(top, before), max(et - kRowDepth, -126)), 121);
             if (m_run == -INFINITY) e_run = e;
             unit_shift = e - et;
             lazy = 0.0f;
