@@ -381,7 +381,8 @@ int sage_paged_gather(const sage_paged_cache* cache, void* k, void* v, const int
                       int64_t tokens, void* stream);
 
 /* Bytes of scratch that sage_paged_attn_fwd needs (the partial results of work split along the
- * keys). Calls that may overlap on the GPU need workspaces of their own. */
+ * keys: 7.5 MB at head_dim 128 where every sequence has few query rows per key/value head, 40 MB and 40
+ * bytes per 256 rows otherwise). Calls that may overlap on the GPU need workspaces of their own. */
 size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q, int64_t batch, int64_t total_q,
                                   int64_t max_seqlen_q, int64_t pages_per_seq);
 
@@ -390,10 +391,14 @@ size_t sage_paged_workspace_bytes(const sage_paged_cache* cache, int64_t heads_q
  * q / o packed [total_q, heads_q, head_dim] with element strides {head, token}; GQA as elsewhere.
  * The query at position p sees key j < seq_lens[b] when j <= p (causal; all keys otherwise) and,
  * with window > 0 (causal only), j > p - window or j < sinks. A query that sees no key gives 0.
- * max_seqlen_q bounds the new tokens of a sequence. o = q (the identical view) is allowed; other
- * overlaps of o are rejected. Keys and values that no query of a sequence sees may hold anything,
- * NaN included; a NaN or infinity in a value that one query sees may reach queries of the same
- * sequence that do not.
+ * max_seqlen_q bounds the new tokens of a sequence and picks the kernels, so the largest number itself serves
+ * best. No sequence may have more: its first max_seqlen_q rows would be taken for its newest, the rest left. sm_scale <= 0 means head_dim ** -0.5. o = q (the
+ * identical view) is allowed; other overlaps of o are rejected. Keys and values that no query of a
+ * sequence sees may hold anything, NaN included; a NaN or infinity in a value that one query sees may
+ * reach queries of the same sequence that do not, a finite one does not, whatever its size. Weights are
+ * rounded to `dtype` (SAGE_CACHE_INT8: times v_scale to fp16, in units of the query's largest such product).
+ * SAGE_CACHE_INT8 forms scores as (q . codes) * k_scale in fp32, q in units of its row's largest value: keys
+ * up to 2^114 in size, queries of any.
  */
 int sage_paged_attn_fwd(const sage_paged_cache* cache, const void* q, const int64_t q_strides[2], void* o,
                         const int64_t o_strides[2], int64_t heads_q, const int32_t* page_table,

@@ -173,3 +173,19 @@ def test_queries_of_any_size(n, log2):
     c["q"] = (c["q"].double() * 2.0 ** log2).to(BF16)
     c["kw"]["k_scale"] *= 2.0 ** -log2
     assert worst(c, run(c)) <= 1
+
+
+@pytest.mark.parametrize("n", [40, 130])
+@pytest.mark.parametrize("span", [10.0, 10.9, 11.1, 12.0])
+@pytest.mark.parametrize("drift", [0, 25, 31, 45, -28, -33, -60])
+def test_where_the_chunk_kernel_changes_its_units(n, span, drift):
+    """Scales spread over 2^span within each tile, and drifting by 2^drift along the sequence: about what one unit per
+    tile takes (2^11), and how far it moves within a segment (2^30)."""
+    past = 1100
+    c = make_case(DEV, new=[n], past=[past], hq=4, hkv=2, dim=64, page=64, dtype=BF16, storage="int8", seed=23)
+    c["kw"]["v_scale"] = torch.where(c["kw"]["v_scale"].isnan(), c["kw"]["v_scale"], 1.0)
+    g = torch.Generator(device=DEV).manual_seed(3)
+    e = span * torch.rand(past + n, generator=g, device=DEV) + drift * torch.arange(past + n, device=DEV) / (past + n)
+    each_scale(c, "v_scale", 2.0 ** (e - 8))
+    assert worst(c, run(c)) <= 1
+    assert worst(c, run(c, window=500, sinks=130), window=500, sinks=130) <= 1

@@ -97,7 +97,7 @@ int paged_move(const sage_paged_cache* c, const void* k, const void* v, const in
   if (!aligned16(k) || !aligned16(v)) return fail(SAGE_ERR_INVALID_ARG, "k/v must be 16-byte aligned");
   for (int i = 0; i < 2; ++i)
     if (ks[i] > (1LL << 33) || vs[i] > (1LL << 33)) return fail(SAGE_ERR_INVALID_ARG, "k/v stride[%d] is too large", i);
-  // what is written must not share a byte with anything else that the call touches
+  // packed tensors must not share a byte with the cache, nor what is read back with itself
   const Span sk = tensor_span(k, k3, 1, c->heads_kv, tokens, c->head_dim, 2);
   const Span sv = tensor_span(v, v3, 1, c->heads_kv, tokens, c->head_dim, 2);
   const Span held[] = {cache_span(c, false), cache_span(c, true), scale_span(c, false), scale_span(c, true)};
@@ -182,16 +182,19 @@ int64_t chunk_items(int64_t batch, int64_t total_q, int64_t G) { return total_q 
 // Which kernel. sage_decode.cuh streams the cache once per 16 query rows of a key/value head, at HBM's
 // rate; sage_chunk.cuh once per 256, at a rate that the softmax of a 128-row tile sets. Above 16 rows the
 // second wins over a 16-bit cache (32 rows over 16 sequences of 20000: 239 instead of 392 us), above 32
-// over an INT8 one, whose codes cost it more (17 to 32 rows: 341 instead of 309 us; 64: 343 instead of
+// over an INT8 one, whose codes cost it more (17 to 32 rows: 341 instead of 311 us; 64: 343 instead of
 // 592).
 int64_t few_rows(const sage_paged_cache* c) { return (c->storage == SAGE_CACHE_INT8 ? 2 : 1) * sage::kDecMaxRows; }
 // Sequences from which two kernels pay: 64 single tokens over up to 8192 beside a chunk of 512, 32/8 heads: 311
 // instead of 377 us (INT8 237 instead of 628); 8 sequences 39 instead of 31 us, the price of two more launches.
 constexpr int64_t kMixedBatch = 16;
 enum class PagedRoute { kFew, kMany, kBoth };
-// Of a batch the host knows the largest sequence's rows and the others' mean. Where the largest has many
-// and the others have few on average (single tokens beside a chunk), both kernels run, each on the
-// sequences of its kind; else the largest decides.
+// Of a batch the host knows a bound on the largest sequence's tokens, and their total. Where the bound means
+// many rows and what it leaves to the others few on average (single tokens beside a chunk), both kernels
+// run, each on the sequences of its kind; else the bound decides. So the bound picks the kernels: with no
+// better one than the total (a caller that does not know its largest sequence) nothing is left to the
+// others, and from 16 sequences on both kernels run, of which one may find no work; and single tokens
+// beside several chunks, whose rows count as the others', go through the many-row kernel.
 PagedRoute paged_route(const sage_paged_cache* c, int64_t G, int64_t batch, int64_t total_q, int64_t max_seqlen_q) {
   const int64_t few = few_rows(c), largest = std::min(max_seqlen_q, total_q);  // a bound may be anything above
   if (largest * G <= few) return PagedRoute::kFew;

@@ -246,8 +246,8 @@ def run_paged_attn(q, cache: PagedKVCache, page_table, seq_lens, cu_seqlens_q=No
     sequence holds) and, with ``window``, j > p - window or j < ``sinks``: the last ``window`` keys, its
     own among them, and the first ``sinks`` ones of the sequence. A query that sees nothing gets o = 0.
     ``max_seqlen_q``: the most new tokens of a sequence (default: total_q, or 1 without
-    ``cu_seqlens_q``); it picks the kernels, so give it where it is known. sm_scale defaults to
-    head_dim ** -0.5. Returns o like q (written into ``out`` when given; ``out=q`` is allowed). The
+    ``cu_seqlens_q``); it picks the kernels, so give it where it is known, and never less than it is (the
+    rows of a sequence that has more are wrong). sm_scale defaults to head_dim ** -0.5. Returns o like q (written into ``out`` when given; ``out=q`` is allowed). The
     scratch of work split along the keys is allocated per call, so calls on several streams or in
     several graphs share nothing.
     """
