@@ -42,7 +42,7 @@
 //
 // Measured (B200, one token of each of 16 sequences of 20000, 64/8 heads, head_dim 128, calls back to back):
 // 16 bit 199 us, 6.58 TB/s, the rate of a plain copy; INT8 118 us, 5.7 TB/s of codes and scales (at 4 sequences
-// of 16000, under the profiler, issue slots 45 % busy, DRAM 48 %). Ragged batches pay for the start and the join:
+// of 16000, under the profiler, issue slots 45 % busy, DRAM 49 %). Ragged batches pay for the start and the join:
 // 64 sequences of 200 to 8192 tokens, 32/8 heads, 16 bit 106 us, 5.6 TB/s. INT8 with 16 rows of an item 171 us (two
 // tokens each), with 32, in two items that each stream the cache, 311 us.
 #pragma once
